@@ -15,14 +15,18 @@ from .allocator import (
     packed_sdm_cow_step,
     packed_sdm_cow_step_layers,
 )
+from .kv_cache import PagedKVCache, PagePlan, prompt_attention
 from .session import DecodeSession
 
 __all__ = [
     "DecodeSession",
+    "PagePlan",
+    "PagedKVCache",
     "PackedSDMCopyOnWriteState",
     "SDMCopyOnWriteStep",
     "dense_sdm_sparse_step",
     "dense_sdm_sparse_step_layers",
     "packed_sdm_cow_step",
     "packed_sdm_cow_step_layers",
+    "prompt_attention",
 ]

@@ -34,6 +34,7 @@ ST_FREE_DUPLICATE = 0x200
 ST_NOT_COVERED = 0x400
 ST_ROW_RANGE = 0x800
 ST_MAP_FULL = 0x1000
+ST_PLAN_TOKENS = 0x2000
 MAP_DENSE, MAP_HASH = 0, 1
 MAX_LAYERS, MAX_WRITES, MAX_READS, MAX_WIDTH = 8, 32, 256, 512
 
@@ -99,6 +100,27 @@ class CowHostPipeline(ctypes.Structure):
         ("h2d_done", c_void_p),
         ("computed", c_void_p),
         ("d2h_done", c_void_p),
+    ]
+
+
+class CowKVPages(ctypes.Structure):
+    _fields_ = [
+        ("key_codes", c_void_p),
+        ("value_codes", c_void_p),
+        ("key_scales", c_void_p),
+        ("value_scales", c_void_p),
+        ("block_tables", c_void_p),
+        ("lengths", c_void_p),
+        ("free_pages", c_void_p),
+        ("free_count", c_void_p),
+        ("status", c_void_p),
+        ("ticket", c_void_p),
+        ("requests", c_int64),
+        ("max_blocks", c_int64),
+        ("pages", c_int64),
+        ("layers", c_int64),
+        ("kv_heads", c_int32),
+        ("width", c_int32),
     ]
 
 
@@ -171,6 +193,14 @@ _SIGNATURES = {
     "cow_pack_apply_layers": (c_int32, [POINTER(CowPool), c_int32, P, c_int64, P]),
     "cow_admit_prefix_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32]),
     "cow_admit_prefix_layers": (c_int32, [POINTER(CowPool), P, P, c_int64, c_int32, P, P, c_int64, P]),
+    "cow_pages_plan_words": (c_int64, [c_int64, c_int64]),
+    "cow_pages_resize": (c_int32, [P, P, c_int64, P, c_int64, P]),
+    "cow_kv8_store": (c_int32, [P, c_int32, P, c_int64, c_int64, P, c_int64, c_int64, c_int32, P, c_int64, P]),
+    "cow_kv8_read": (c_int32, [P, c_int32, P, c_int64, P, P, c_int32, P]),
+    "cow_kv8_attend_workspace_bytes": (c_int64, [P, c_int32]),
+    "cow_kv8_attend": (c_int32, [P, c_int32, P, c_int64, c_int64, c_int32, c_int32, ctypes.c_float, P, P, c_int64, P]),
+    "cow_prompt_attention": (c_int32, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64,
+                                       c_int64, c_int32, c_int32, c_int32, c_int32, ctypes.c_float, P, P]),
     "cow_validate_workspace_bytes": (c_int64, [POINTER(CowPool), c_int32]),
     "cow_validate_layers": (c_int32, [POINTER(CowPool), c_int32, P, c_int64, P, P]),
 }

@@ -740,7 +740,8 @@ inline size_t read_stage_bytes(int reads, int64_t width, int ch, int rv, int dty
 
 // Blocks of `fn` (with `smem` dynamic shared memory) that fit on the current
 // device at once, cached per device / kernel / size; raises the kernel's
-// dynamic shared memory limit when it needs more than the default 48 KiB.
+// dynamic shared memory limit when it needs more than the default 48 KiB (and
+// never lowers it below what an earlier, cached size needs).
 inline int resident_blocks(const void* fn, int threads, size_t smem) {
   struct Entry {
     int device;
@@ -754,10 +755,14 @@ inline int resident_blocks(const void* fn, int threads, size_t smem) {
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return 0;
   std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < used; ++i)
-    if (cache[i].device == device && cache[i].fn == fn && cache[i].smem == smem) return cache[i].blocks;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) {
+  size_t limit = smem;
+  for (int i = 0; i < used; ++i) {
+    if (cache[i].device != device || cache[i].fn != fn) continue;
+    if (cache[i].smem == smem) return cache[i].blocks;
+    if (cache[i].smem > limit) limit = cache[i].smem;
+  }
+  if (limit > 48 * 1024 &&
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(limit)) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }

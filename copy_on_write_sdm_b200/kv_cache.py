@@ -1,0 +1,370 @@
+"""Serving operators of the dense attention layers: a prompt's attention, and a paged
+K/V cache held in 8 bits with the attention of single tokens over it.
+
+* ``prompt_attention``: causal attention over packed prompts of different lengths,
+  grouped heads, one launch;
+* ``PagedKVCache``: pages of 64 tokens from one stack shared by all requests and layers,
+  taken and returned in a deterministic order as the SDM pools take rows.  ``resize`` moves
+  every request to a target length and gives the block tables and slot maps of the new
+  tokens, ``store`` quantises their keys and values, ``attend`` answers one query token
+  per request, ``read`` gives stored values back.
+
+The reference keeps a fixed-capacity cache in the activation type for these layers
+(copy_on_write_sdm/inference.py:293-306, model.py:127-185) and has no counterpart.
+Serving only: no operator here has a backward pass, and inputs that ask for one are refused.
+Every operation runs through ``libcowsdm.so`` (sm_100a) on the current stream; it
+neither synchronises nor allocates anything but its results and, once, its workspace.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field, replace
+from typing import Sequence
+
+import torch
+
+from . import _lib
+
+PAGE_TOKENS = 64
+MAX_REQUESTS = 8192
+HEAD_WIDTHS = (32, 64, 96, 128)
+MAX_GROUP = 64  # query heads to a key head, prompt attention
+
+_STATUS_TEXT = [
+    (_lib.ST_SLAB_EXHAUSTED, "the K/V cache has no free page left"),
+    (_lib.ST_INDEX_RANGE, "a request's length lies outside its block table"),
+    (_lib.ST_PLAN_TOKENS, "a resize adds more tokens than were announced"),
+    (_lib.ST_ROW_RANGE, "a block table holds no page for a cached token"),
+]
+
+
+def _on_device(device: torch.device):
+    """The device made current for a call, where it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return None
+    return torch.cuda.device(device)
+
+
+def _call(device: torch.device, what: str, *args) -> None:
+    fn = getattr(_lib.load(), what)
+    guard = _on_device(device)
+    if guard is None:
+        rc = fn(*args, _lib.stream_of(device))
+    else:
+        with guard:
+            rc = fn(*args, _lib.stream_of(device))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` with rows the kernels can read: contiguous, on 16-byte boundaries (a copy where it is not so)."""
+    if not t.is_cuda:
+        _lib.require_cuda(t, what)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} asks for a gradient: the serving attention has no backward pass")
+    size = t.element_size()
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and not (s0 * size) % 16 and not (s1 * size) % 16 and not t.data_ptr() % 16:
+        return t
+    t = t.contiguous()
+    return t if not t.data_ptr() % 16 else t.clone()
+
+
+def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, starts: torch.Tensor, *,
+                     scale: float | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts.
+
+    ``queries`` ``[tokens, heads, width]``, ``keys`` and ``values`` ``[tokens, kv_heads,
+    width]`` (float32, bfloat16 or float16, any strides with contiguous rows); sequence b
+    holds tokens ``starts[b] .. starts[b+1]-1`` (int32, ascending, on the device).  Token i
+    attends to its own sequence's tokens up to itself with ``softmax(scale * q . k)``, ``scale``
+    1 / sqrt(width) by default; ``heads / kv_heads`` neighbouring query heads share a key head.
+    Returns ``[tokens, heads, width]``; rows of tokens outside every sequence are unspecified.
+    """
+    if queries.ndim != 3 or keys.ndim != 3 or keys.shape != values.shape:
+        raise ValueError("prompt attention takes queries, keys and values [tokens, heads, width]")
+    tokens, heads, width = queries.shape
+    kv_heads = keys.shape[1]
+    if keys.shape[0] != tokens or keys.shape[2] != width or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("queries, keys and values do not match")
+    if heads < 1 or width < 1 or width % 8 or width > 128 or heads // kv_heads > MAX_GROUP:
+        raise ValueError(f"prompt attention takes widths of 8, 16 .. 128 and up to {MAX_GROUP} query heads to a key head")
+    if not queries.dtype == keys.dtype == values.dtype:
+        raise ValueError("queries, keys and values must share one dtype")
+    code = _lib.dtype_code(queries.dtype)
+    q, k, v = _rows(queries, "queries"), _rows(keys, "keys"), _rows(values, "values")
+    device = q.device
+    if k.device != device or v.device != device or starts.device != device:
+        raise ValueError("queries, keys, values and starts must be on one device")
+    if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 1 or not starts.is_contiguous():
+        raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
+    out = torch.empty((tokens, heads, width), dtype=q.dtype, device=device)
+    _call(device, "cow_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+          v.data_ptr(), v.stride(0), v.stride(1), starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
+          code, width ** -0.5 if scale is None else float(scale), out.data_ptr())
+    return out
+
+
+class PagePlan:
+    """Where a resize put the new tokens: ``starts`` ``[requests + 1]`` (their packed
+    order, request by request), ``slots`` and ``positions`` ``[tokens]`` (``64 * page +
+    offset`` in the cache, place in the request; -1 past the new tokens), all int32 on
+    the device, and ``pieces`` (the new tokens page by page) for ``store``."""
+
+    __slots__ = ("cache", "epoch", "requests", "tokens", "buffer", "_at")
+
+    def __init__(self, cache: "PagedKVCache", epoch: int, tokens: int, buffer: torch.Tensor) -> None:
+        self.cache, self.epoch, self.tokens, self.buffer = cache, epoch, tokens, buffer
+        self.requests = cache.requests
+        self._at = buffer.numel() - (self.requests + 1 + 2 * tokens)
+
+    @property
+    def starts(self) -> torch.Tensor:
+        return self.buffer[self._at:self._at + self.requests + 1]
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self.buffer[self._at + self.requests + 1:self._at + self.requests + 1 + self.tokens]
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self.buffer[self.buffer.numel() - self.tokens:]
+
+    @property
+    def pieces(self) -> torch.Tensor:
+        """``[max pieces, 4]``: first packed token, tokens, page, offset; the first ``buffer[0]`` are set."""
+        return self.buffer[4:self._at].view(-1, 4)
+
+
+@dataclass(frozen=True, eq=False)
+class PagedKVCache:
+    """K/V of a batch of requests for ``layers`` attention layers, in pages of 64 tokens.
+
+    Keys and values are e4m3 codes with one power-of-two scale per (layer, page, head): a
+    value is ``code * scale``.  ``value_pages`` hold a page's tokens side by side.  A page
+    id stands for one page in every layer, so one ``resize`` serves them all.
+    ``free_pages`` is a stack with its top at ``free_count - 1``.  ``status_word`` collects
+    device errors as the SDM pools' ``overflow_flag`` does; ``validate_invariants`` raises.
+    """
+
+    key_pages: torch.Tensor      # [layers, pages, kv_heads, 64, head_width] float8_e4m3fn
+    value_pages: torch.Tensor    # [layers, pages, kv_heads, head_width, 64] float8_e4m3fn
+    key_scales: torch.Tensor     # [layers, pages, kv_heads] float32
+    value_scales: torch.Tensor   # [layers, pages, kv_heads] float32
+    block_tables: torch.Tensor   # [requests, max_blocks] int32
+    lengths: torch.Tensor        # [requests] int32
+    free_pages: torch.Tensor     # [pages] int32
+    free_count: torch.Tensor     # int32
+    status_word: torch.Tensor    # int32
+    ticket: torch.Tensor         # int32
+    _epoch: list = field(default_factory=lambda: [0], repr=False)
+    _own: dict = field(default_factory=dict, repr=False, init=False)
+
+    @classmethod
+    def allocate(cls, *, requests: int, pages: int, kv_heads: int, head_width: int, max_blocks: int, layers: int = 1,
+                 device: torch.device | str = "cuda") -> "PagedKVCache":
+        """An empty cache: ``requests`` block tables of ``max_blocks`` pages of 64 tokens, over ``pages`` pages."""
+        if requests < 0 or pages < 0 or kv_heads < 1 or max_blocks < 0 or layers < 1:
+            raise ValueError("K/V cache sizes are invalid")
+        if head_width not in HEAD_WIDTHS:
+            raise ValueError(f"the 8-bit K/V cache takes head widths {HEAD_WIDTHS}")
+        if requests > MAX_REQUESTS or requests * max_blocks >= 1 << 25 or pages >= 1 << 25 or kv_heads > 1024:
+            raise ValueError("the K/V cache exceeds the compiled limits (8192 requests, 2^25 pages and table entries)")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("the paged K/V cache must be on a CUDA device: it runs only through the sm_100a kernels")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+
+        def zeros(*shape, dtype=torch.int32):
+            return torch.zeros(shape, dtype=dtype, device=device)
+
+        codes = (layers, pages, kv_heads, PAGE_TOKENS, head_width)
+        return cls(
+            key_pages=zeros(*codes, dtype=torch.uint8).view(torch.float8_e4m3fn),
+            value_pages=zeros(layers, pages, kv_heads, head_width, PAGE_TOKENS, dtype=torch.uint8).view(torch.float8_e4m3fn),
+            key_scales=zeros(layers, pages, kv_heads, dtype=torch.float32),
+            value_scales=zeros(layers, pages, kv_heads, dtype=torch.float32),
+            block_tables=torch.full((requests, max_blocks), -1, dtype=torch.int32, device=device),
+            lengths=zeros(requests), free_pages=torch.arange(pages, dtype=torch.int32, device=device),
+            free_count=torch.tensor(pages, dtype=torch.int32, device=device), status_word=zeros(), ticket=zeros())
+
+    # ---- sizes
+
+    @property
+    def device(self) -> torch.device:
+        return self.lengths.device
+
+    @property
+    def requests(self) -> int:
+        return self.lengths.shape[0]
+
+    @property
+    def layers(self) -> int:
+        return self.key_pages.shape[0]
+
+    @property
+    def pages(self) -> int:
+        return self.key_pages.shape[1]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.key_pages.shape[2]
+
+    @property
+    def head_width(self) -> int:
+        return self.key_pages.shape[4]
+
+    @property
+    def max_blocks(self) -> int:
+        return self.block_tables.shape[1]
+
+    def storage_bytes(self) -> dict[str, int]:
+        """Bytes reserved for codes and scales, and for tables and stack."""
+        pools = (self.key_pages, self.value_pages, self.key_scales, self.value_scales)
+        meta = (self.block_tables, self.lengths, self.free_pages, self.free_count, self.status_word, self.ticket)
+        return {"kv_pages": sum(t.numel() * t.element_size() for t in pools),
+                "kv_metadata": sum(t.numel() * t.element_size() for t in meta)}
+
+    def _desc(self) -> int:
+        """Address of the C descriptor; the tensors it points to are fixed for this object's life."""
+        at = self._own.get("at")
+        if at is None:
+            desc = _lib.CowKVPages(
+                *(t.data_ptr() for t in (self.key_pages, self.value_pages, self.key_scales, self.value_scales,
+                                         self.block_tables, self.lengths, self.free_pages, self.free_count,
+                                         self.status_word, self.ticket)),
+                self.requests, self.max_blocks, self.pages, self.layers, self.kv_heads, self.head_width)
+            self._own["desc"] = desc
+            at = self._own["at"] = ctypes.addressof(desc)
+        return at
+
+    # ---- operators
+
+    def resize(self, targets: torch.Tensor | Sequence[int], *, tokens: int) -> PagePlan:
+        """Move every request to its target length (int32 ``[requests]``), in one launch.
+
+        Requests that shrink give their last pages back first; requests that grow then take
+        pages, request by request and block by block, from the stack's top.  ``tokens``
+        is the number of new tokens in all, or a bound on it (the plan's size).  A target
+        that does not fit the block table or the stack, or more new tokens than ``tokens``,
+        changes nothing, plans nothing and sets ``status_word``.
+        """
+        if not isinstance(targets, torch.Tensor):
+            targets = torch.tensor(targets, dtype=torch.int32, device=self.device)
+        if targets.dtype != torch.int32 or targets.ndim != 1 or targets.shape[0] != self.requests \
+                or targets.device != self.device or not targets.is_contiguous():
+            raise ValueError("targets must be a contiguous int32 vector [requests] on the cache's device")
+        words = _lib.load().cow_pages_plan_words(self.requests, int(tokens))
+        if words < 0:
+            raise ValueError("the number of new tokens is invalid")
+        self._epoch[0] += 1
+        plan = PagePlan(self, self._epoch[0], int(tokens), torch.empty(words, dtype=torch.int32, device=self.device))
+        _call(self.device, "cow_pages_resize", self._desc(), targets.data_ptr(), plan.tokens, plan.buffer.data_ptr(), words)
+        return plan
+
+    def store(self, keys: torch.Tensor, values: torch.Tensor, plan: PagePlan, *, layer: int = 0) -> None:
+        """Quantise the plan's new tokens' ``keys`` and ``values`` ``[tokens, kv_heads, head_width]`` into ``layer``.
+
+        The scale of a page and head is the smallest power of two with ``max|x| <= 448 * scale``
+        over its tokens; a page that already holds tokens keeps its scale where that is larger, and
+        has its codes rounded again to a larger one.  Infinities become the largest code.
+        """
+        shape = (plan.tokens, self.kv_heads, self.head_width)
+        if keys.shape != shape or values.shape != shape:
+            raise ValueError(f"stored keys and values must be {list(shape)}")
+        if plan.cache._epoch is not self._epoch or plan.epoch != self._epoch[0]:
+            raise ValueError("the plan is not of this cache's last resize")
+        if keys.dtype != values.dtype:
+            raise ValueError("keys and values must share one dtype")
+        if not 0 <= layer < self.layers:
+            raise ValueError("the K/V cache has no such layer")
+        k, v = _rows(keys, "keys"), _rows(values, "values")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError("keys and values must be on the cache's device")
+        _call(self.device, "cow_kv8_store", self._desc(), layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+              v.stride(0), v.stride(1), _lib.dtype_code(k.dtype), plan.buffer.data_ptr(), plan.tokens)
+
+    def read(self, slots: torch.Tensor, *, layer: int = 0, dtype: torch.dtype = torch.bfloat16):
+        """Keys and values ``[slots, kv_heads, head_width]`` that the cache holds at ``slots`` (int32; zeros for -1)."""
+        if slots.dtype != torch.int32 or slots.ndim != 1 or slots.device != self.device or not slots.is_contiguous():
+            raise ValueError("slots must be a contiguous int32 vector on the cache's device")
+        if not 0 <= layer < self.layers:
+            raise ValueError("the K/V cache has no such layer")
+        code = _lib.dtype_code(dtype)
+        out = torch.empty((2, slots.shape[0], self.kv_heads, self.head_width), dtype=dtype, device=self.device)
+        keys, values = out[0], out[1]
+        _call(self.device, "cow_kv8_read", self._desc(), layer, slots.data_ptr(), slots.shape[0], keys.data_ptr(),
+              values.data_ptr(), code)
+        return keys, values
+
+    def attend(self, queries: torch.Tensor, *, layer: int = 0, scale: float | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """One query token per request over its cached tokens, ``[requests, heads, head_width]``.
+
+        ``softmax(scale * q . K) V`` in float32 over the ``lengths[b]`` cached tokens, ``scale`` 1 /
+        sqrt(head_width) by default; zeros for a request without tokens.  Calls that may overlap
+        on the GPU need a ``workspace`` each (``new_workspace``).
+        """
+        if queries.ndim != 3 or queries.shape[0] != self.requests or queries.shape[2] != self.head_width \
+                or queries.shape[1] < 1 or queries.shape[1] % self.kv_heads:
+            raise ValueError("attend takes queries [requests, heads, head_width], heads a multiple of kv_heads")
+        if not 0 <= layer < self.layers:
+            raise ValueError("the K/V cache has no such layer")
+        code = _lib.dtype_code(queries.dtype)
+        q = _rows(queries, "queries")
+        if q.device != self.device:
+            raise ValueError("queries must be on the cache's device")
+        heads = q.shape[1]
+        if workspace is None:
+            workspace = self._own.get(heads)
+            if workspace is None:
+                workspace = self._own[heads] = self.new_workspace(heads)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _call(self.device, "cow_kv8_attend", self._desc(), layer, q.data_ptr(), q.stride(0), q.stride(1), code, heads,
+              self.head_width ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),
+              workspace.numel())
+        return out
+
+    def new_workspace(self, heads: int) -> torch.Tensor:
+        """A zero-filled workspace of ``attend`` for ``heads`` query heads."""
+        need = _lib.load().cow_kv8_attend_workspace_bytes(self._desc(), heads)
+        if need < 0:
+            raise ValueError("heads must be a multiple of kv_heads")
+        return torch.zeros(need, dtype=torch.uint8, device=self.device)
+
+    # ---- lifecycle
+
+    def with_requests(self, keep: torch.Tensor | Sequence[int], *, new: int = 0) -> "PagedKVCache":
+        """The cache with the request slots ``keep``, in their order, and ``new`` empty ones after
+        them: same pages and stack.  Requests left out must have been resized to 0 (their pages
+        would be lost).  The old object is not used again."""
+        keep = torch.as_tensor(keep, dtype=torch.int64, device=self.device)
+        total = keep.shape[0] + new
+        if new < 0 or total > MAX_REQUESTS or total * self.max_blocks >= 1 << 25:
+            raise ValueError("the K/V cache exceeds the compiled limits (8192 requests, 2^25 table entries)")
+        tables = self.block_tables.new_full((total, self.max_blocks), -1)
+        lengths = self.lengths.new_zeros(total)
+        tables[:keep.shape[0]] = self.block_tables[keep]
+        lengths[:keep.shape[0]] = self.lengths[keep]
+        self._epoch[0] += 1  # plans made for the old slots are over
+        return replace(self, block_tables=tables, lengths=lengths)
+
+    def validate_invariants(self) -> None:
+        """Raise on a device error, or where live and free pages do not partition the pool (synchronises)."""
+        bits = int(self.status_word.item())
+        if bits:
+            raise RuntimeError("; ".join(text for bit, text in _STATUS_TEXT if bits & bit) or f"K/V cache status {bits}")
+        blocks = (self.lengths.long() + PAGE_TOKENS - 1) // PAGE_TOKENS
+        live = torch.arange(self.max_blocks, device=self.device) < blocks[:, None]
+        if bool(((self.block_tables >= 0) != live).any()):
+            raise AssertionError("K/V block tables do not match the lengths")
+        count = int(self.free_count.item())
+        if not 0 <= count <= self.pages:
+            raise AssertionError("K/V free page count is invalid")
+        every = torch.cat((self.block_tables[live], self.free_pages[:count]))
+        if every.numel() != self.pages or not torch.equal(every.sort().values.long(),
+                                                          torch.arange(self.pages, device=self.device)):
+            raise AssertionError("live and free K/V pages do not partition the cache")

@@ -55,6 +55,7 @@ extern "C" {
 #define COW_ST_NOT_COVERED 0x400      /* validate: a row is neither live nor free */
 #define COW_ST_ROW_RANGE 0x800        /* validate: a map / stack entry lies outside capacity */
 #define COW_ST_MAP_FULL 0x1000        /* a hashed map's bank table had no empty entry for a first touch */
+#define COW_ST_PLAN_TOKENS 0x2000     /* a resize adds more tokens than its plan has room for */
 
 #define COW_MAX_LAYERS 8
 #define COW_MAX_WRITES 32
@@ -538,6 +539,106 @@ int cow_attention_mlp_decode(const float* tokens, const int64_t* positions, cons
                              const float* mlp_norm_weight, const float* mlp_norm_bias, float mlp_eps,
                              const float* mlp_in_weight_t, const float* mlp_out_weight_t, int64_t batch,
                              int32_t width, int32_t heads, int32_t hidden, float* out, void* stream);
+
+/* ---- paged 8-bit K/V cache of the dense attention layers ------------------
+ *
+ * No counterpart in the reference, whose dense layers keep a fixed-capacity
+ * cache in the activation type (copy_on_write_sdm/inference.py:293-306).
+ * Pages of COW_PAGE_TOKENS tokens come from one stack that all layers share
+ * (a page id stands for one page of every layer):
+ *   key_codes    [layers, pages, kv_heads, 64, width]  e4m3
+ *   value_codes  [layers, pages, kv_heads, width, 64]  e4m3, a page's tokens side by side
+ *   key_scales, value_scales [layers, pages, kv_heads] float32, powers of two
+ *   block_tables [requests, max_blocks] int32          page of each block, -1 none
+ *   lengths      [requests] int32                      cached tokens
+ *   free_pages   [pages] int32                         free stack, top at free_pages[free_count-1]
+ *   free_count, status, ticket   int32 device scalars (ticket: zero, left zero)
+ * A value is code * scale of its page and head.  width is 32, 64, 96 or 128;
+ * requests <= 8192, requests * max_blocks < 2^25, pages < 2^25.  Calls on one
+ * cache that could overlap on the GPU are the caller's to order. */
+#define COW_PAGE_TOKENS 64
+#define COW_MAX_REQUESTS 8192
+
+typedef struct cow_kv_pages {
+  uint8_t* key_codes;
+  uint8_t* value_codes;
+  float* key_scales;
+  float* value_scales;
+  int32_t* block_tables;
+  int32_t* lengths;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int32_t* status;
+  int32_t* ticket;
+  int64_t requests, max_blocks, pages, layers;
+  int32_t kv_heads, width;
+} cow_kv_pages;
+
+/* Moves every request to targets[b] (device int32) cached tokens, in one
+ * launch: pages past a shorter target return to the stack, then longer targets
+ * take pages, request by request and block by block: the r-th taken is
+ * free_pages[top-1-r], and freed pages lie so that the first freed is the next
+ * taken.  The plan (cow_pages_plan_words(requests, tokens) int32 words, 16-byte
+ * aligned) receives, in this order:
+ *   [4]               pieces, new tokens, 0, 0
+ *   [4 * max pieces]  per piece (new tokens of one page): first packed token,
+ *                     tokens, page, offset in the page;
+ *                     max pieces = min(tokens, tokens / 64 + 2 * requests)
+ *   [requests + 1]    starts: exclusive prefix of each request's new tokens
+ *   [tokens]          slots: 64 * page + offset of each new token, packed
+ *   [tokens]          positions of the new tokens in their requests
+ * Room past the new tokens is filled with -1.  A target outside
+ * [0, 64 * max_blocks], more new tokens than `tokens`, or a stack without
+ * enough pages sets COW_ST_INDEX_RANGE, COW_ST_PLAN_TOKENS or
+ * COW_ST_SLAB_EXHAUSTED, plans nothing and changes nothing. */
+int64_t cow_pages_plan_words(int64_t requests, int64_t tokens);
+int cow_pages_resize(const cow_kv_pages* cache, const int32_t* targets, int64_t tokens, int32_t* plan,
+                     int64_t plan_words, void* stream);
+
+/* Quantises the plan's new tokens' keys and values ([tokens, kv_heads, width]
+ * in dtype, strides in elements, rows of `width` contiguous, 16-byte aligned)
+ * into layer `layer`.  Per page and head the scale is the smallest 2^e >= 2^-64
+ * with max|x| <= 448 * 2^e over the finite values stored, not below the page's
+ * own scale if it holds tokens already (whose codes are rounded again to a
+ * larger one); codes are x / scale to nearest even, infinities +-448, NaN NaN.
+ * A plan is stored at most once per layer before the next resize of the cache
+ * (storing it again writes the same). */
+int cow_kv8_store(const cow_kv_pages* cache, int32_t layer, const void* keys, int64_t key_token_stride,
+                  int64_t key_head_stride, const void* values, int64_t value_token_stride, int64_t value_head_stride,
+                  int32_t dtype, const int32_t* plan, int64_t tokens, void* stream);
+
+/* The values that the cache holds at `slots` [count]: keys and values
+ * [count, kv_heads, width] in dtype; zeros for a slot outside the cache. */
+int cow_kv8_read(const cow_kv_pages* cache, int32_t layer, const int32_t* slots, int64_t count, void* keys,
+                 void* values, int32_t dtype, void* stream);
+
+/* One query token per request over its cached tokens:
+ *   o = softmax(scale * q . K) V per query head, heads / kv_heads query heads
+ * sharing a key and value head; a request without tokens gives zeros.  queries
+ * [requests, heads, width] in dtype (strides in elements, rows contiguous,
+ * 16-byte aligned), out contiguous.  The workspace is
+ * cow_kv8_attend_workspace_bytes bytes (-1: bad arguments), zero-filled before
+ * its first use, 16-byte aligned, and left ready for the next call; calls that
+ * may overlap on the GPU need separate ones. */
+int64_t cow_kv8_attend_workspace_bytes(const cow_kv_pages* cache, int32_t heads);
+int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries, int64_t query_request_stride,
+                   int64_t query_head_stride, int32_t dtype, int32_t heads, float scale, void* out, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* Causal attention over packed prompts: sequence b holds tokens
+ * starts[b]..starts[b+1]-1 (device int32 [sequences + 1], ascending), token i
+ * attends to the tokens of its sequence up to itself:
+ *   o_i = softmax_j(scale * q_i . k_j) v_j
+ * queries, out [tokens, heads, width], keys, values [tokens, kv_heads, width]
+ * in dtype; strides in elements, rows contiguous and 16-byte aligned, out
+ * contiguous.  width a multiple of 8 up to 128, heads a multiple of kv_heads
+ * with at most 64 query heads to a key head.  Tokens outside every sequence
+ * are not written. */
+int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_t query_head_stride,
+                         const void* keys, int64_t key_token_stride, int64_t key_head_stride, const void* values,
+                         int64_t value_token_stride, int64_t value_head_stride, const int32_t* starts,
+                         int64_t sequences, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t width,
+                         int32_t dtype, float scale, void* out, void* stream);
 
 /* materialize_dense (allocator.py:1004-1017): dense [banks,slots,width] in out_dtype. */
 int cow_materialize(const cow_pool* pool, void* out, int32_t out_dtype, void* stream);
