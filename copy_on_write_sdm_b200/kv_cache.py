@@ -58,18 +58,23 @@ def _call(device: torch.device, what: str, *args) -> None:
         _lib.check(rc, what)
 
 
-def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
-    """``t`` with rows the kernels can read: contiguous, on 16-byte boundaries (a copy where it is not so)."""
+def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
+    """``t`` [n, heads, width] with rows the kernels can read, contiguous and on 16-byte boundaries (a
+    copy where it is not so), and its strides; those of a dimension of one are made up."""
     if not t.is_cuda:
         _lib.require_cuda(t, what)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} asks for a gradient: the serving attention has no backward pass")
-    size = t.element_size()
+    n, heads, width = t.shape
     s0, s1, s2 = t.stride()
-    if s2 == 1 and not (s0 * size) % 16 and not (s1 * size) % 16 and not t.data_ptr() % 16:
-        return t
-    t = t.contiguous()
-    return t if not t.data_ptr() % 16 else t.clone()
+    if heads == 1:
+        s1 = width
+    if n == 1:
+        s0 = heads * width
+    mask = 3 if t.element_size() == 4 else 7
+    if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & mask and not t.data_ptr() & 15:
+        return t, s0, s1
+    return t.clone(memory_format=torch.contiguous_format), heads * width, width
 
 
 def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, starts: torch.Tensor, *,
@@ -94,15 +99,14 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     if not queries.dtype == keys.dtype == values.dtype:
         raise ValueError("queries, keys and values must share one dtype")
     code = _lib.dtype_code(queries.dtype)
-    q, k, v = _rows(queries, "queries"), _rows(keys, "keys"), _rows(values, "values")
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(queries, "queries"), _rows(keys, "keys"), _rows(values, "values")
     device = q.device
     if k.device != device or v.device != device or starts.device != device:
         raise ValueError("queries, keys, values and starts must be on one device")
     if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
     out = torch.empty((tokens, heads, width), dtype=q.dtype, device=device)
-    _call(device, "cow_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-          v.data_ptr(), v.stride(0), v.stride(1), starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
+    _call(device, "cow_prompt_attention", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
           code, width ** -0.5 if scale is None else float(scale), out.data_ptr())
     return out
 
@@ -281,11 +285,10 @@ class PagedKVCache:
             raise ValueError("keys and values must share one dtype")
         if not 0 <= layer < self.layers:
             raise ValueError("the K/V cache has no such layer")
-        k, v = _rows(keys, "keys"), _rows(values, "values")
+        (k, k0, k1), (v, v0, v1) = _rows(keys, "keys"), _rows(values, "values")
         if k.device != self.device or v.device != self.device:
             raise ValueError("keys and values must be on the cache's device")
-        _call(self.device, "cow_kv8_store", self._desc(), layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-              v.stride(0), v.stride(1), _lib.dtype_code(k.dtype), plan.buffer.data_ptr(), plan.tokens)
+        _call(self.device, "cow_kv8_store", self._desc(), layer, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, _lib.dtype_code(k.dtype), plan.buffer.data_ptr(), plan.tokens)
 
     def read(self, slots: torch.Tensor, *, layer: int = 0, dtype: torch.dtype = torch.bfloat16):
         """Keys and values ``[slots, kv_heads, head_width]`` that the cache holds at ``slots`` (int32; zeros for -1)."""
@@ -314,7 +317,7 @@ class PagedKVCache:
         if not 0 <= layer < self.layers:
             raise ValueError("the K/V cache has no such layer")
         code = _lib.dtype_code(queries.dtype)
-        q = _rows(queries, "queries")
+        q, q0, q1 = _rows(queries, "queries")
         if q.device != self.device:
             raise ValueError("queries must be on the cache's device")
         heads = q.shape[1]
@@ -323,7 +326,7 @@ class PagedKVCache:
             if workspace is None:
                 workspace = self._own[heads] = self.new_workspace(heads)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _call(self.device, "cow_kv8_attend", self._desc(), layer, q.data_ptr(), q.stride(0), q.stride(1), code, heads,
+        _call(self.device, "cow_kv8_attend", self._desc(), layer, q.data_ptr(), q0, q1, code, heads,
               self.head_width ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),
               workspace.numel())
         return out

@@ -596,7 +596,7 @@ int cow_pages_resize(const cow_kv_pages* cache, const int32_t* targets, int64_t 
                      int64_t plan_words, void* stream);
 
 /* Quantises the plan's new tokens' keys and values ([tokens, kv_heads, width]
- * in dtype, strides in elements, rows of `width` contiguous, 16-byte aligned)
+ * in dtype, strides in elements, positive, rows of `width` contiguous, 16-byte aligned)
  * into layer `layer`.  Per page and head the scale is the smallest 2^e >= 2^-64
  * with max|x| <= 448 * 2^e over the finite values stored, not below the page's
  * own scale if it holds tokens already (whose codes are rounded again to a
@@ -630,7 +630,7 @@ int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries
  * attends to the tokens of its sequence up to itself:
  *   o_i = softmax_j(scale * q_i . k_j) v_j
  * queries, out [tokens, heads, width], keys, values [tokens, kv_heads, width]
- * in dtype; strides in elements, rows contiguous and 16-byte aligned, out
+ * in dtype; strides in elements, positive, rows contiguous and 16-byte aligned, out
  * contiguous.  width a multiple of 8 up to 128, heads a multiple of kv_heads
  * with at most 64 query heads to a key head.  Tokens outside every sequence
  * are not written. */
