@@ -229,12 +229,13 @@ __global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_c
 // 16-bit types: tcgen05
 // --------------------------------------------------------------------------
 //
-// A block has two tiles A and B of 128 rows against key tiles of 128 tokens, twelve warps:
-//   warps 0-3, 4-7   softmax of A and of B: a thread owns a row, so maximum and sum need no exchange
-//   warp 8           one thread loads by TMA: the query tiles once, K and V tiles round a ring
-//   warp 9           one thread issues the products: S = Q K^T into tensor memory, and O += P V
+// A block has two tiles A and B of 128 rows against key tiles of 128 tokens, twenty warps:
+//   warps 0-7, 8-15  softmax of A and of B: two threads to a row, 64 keys each, so that the row's scores
+//                    fit registers with four warps to a scheduler; the two meet once a key tile
+//   warp 16          one thread loads by TMA: the query tiles once, K and V tiles round a ring
+//   warp 17          one thread issues the products: S = Q K^T into tensor memory, and O += P V
 //                    with P read from tensor memory, where it takes the place of S
-//   warps 10, 11     look through the values of masked tiles (below)
+//   warp 18          looks through the values of masked tiles (below)
 // While one tile's softmax runs, the tensor cores work on the other's O += P V and next S; S(j + 1) of a
 // tile is issued after O += P V (j) of it, so its arrival also says that O may be touched.
 // O lies in tensor memory for the whole pass.  It is rescaled only when a row's maximum has grown by more
@@ -249,18 +250,19 @@ __global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_c
 //
 // Every wait is bounded; one that gives up ends the block with NaN rows.
 
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 640;
 constexpr int kTcRows = 128;  // rows of a tile
 constexpr int kTcKeys = 128;  // tokens of a key tile
 constexpr int kTcLimit = 1 << 18;
 constexpr float kLazy = 8.f;  // log2 of the growth of a maximum that is let pass
 
-template <int DP>  // width rounded up to 64s
+template <int DP>  // width rounded up to 32s
 struct TcShape {
-  static constexpr int kParts = DP / 64;                        // 128-byte wide parts of a row
+  static constexpr int kParts = (DP + 63) / 64;                        // 128-byte wide parts of a row
   static constexpr int kPartBytes = 128 * 128;                  // 128 rows of one part
   static constexpr int kTileBytes = kParts * kPartBytes;
-  static constexpr int kSlots = DP == 128 ? 4 : 8;              // ring of K and V tiles
+  static constexpr int kSlots = DP > 64 ? 4 : 8;                // ring of K and V tiles
+  static constexpr int kPoly = DP > 64 ? 2 : 3;                 // of 8 pairs of weights, those from the polynomial
   static constexpr int kBytes = (2 + kSlots) * kTileBytes + 1024;
 };
 
@@ -271,9 +273,27 @@ struct TcLaunch {
 
 struct TcBarriers {
   uint64_t full[8], empty[8];
-  uint64_t q, s[2], p[2], o[2], look[2], looked[2], drain;  // look, looked: at most two tiles are masked
+  uint64_t q, s[2], p[2][2], o[2], look[2], looked[2], drain;  // look, looked: at most two tiles are masked
 };
 
+// Two warps (64 threads) at named barrier `id`: whether `yes` holds in any of their threads; a plain meeting.
+__device__ __forceinline__ bool any_of_two_warps(int id, bool yes) {
+  unsigned any;
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred q, %2, 64, p; selp.u32 %0, 1, 0, q; }"
+      : "=r"(any)
+      : "r"(static_cast<unsigned>(yes)), "r"(id)
+      : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void two_warps_meet(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// One thread of a converged warp, known to the compiler to be one.
+__device__ __forceinline__ bool elect_one() {
+  unsigned one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -321,6 +341,18 @@ __device__ __forceinline__ void tc_store32(unsigned at, const unsigned* r) {
       COW_W8(r, 8), COW_W8(r, 16), COW_W8(r, 24), "r"(at)
       : "memory");
 }
+__device__ __forceinline__ void tc_load8(unsigned at, unsigned* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : COW_R8(r, 0) : "r"(at));
+}
+__device__ __forceinline__ void tc_store8(unsigned at, const unsigned* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::COW_W8(r, 0), "r"(at) : "memory");
+}
+__device__ __forceinline__ void tc_store16(unsigned at, const unsigned* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::COW_W8(r, 0),
+      COW_W8(r, 8), "r"(at)
+      : "memory");
+}
 #undef COW_R8
 #undef COW_W8
 __device__ __forceinline__ void tc_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -343,11 +375,66 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
     return *reinterpret_cast<const unsigned*>(&h);
   }
 }
+// pairs of floats in one 64-bit register
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t r) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^y of both halves on the multiply-add pipe, for y <= about 100: with n the nearest integer, f = y - n in
+// [-1/2, 1/2] and 2^f a polynomial with constant term 1, fitted here by reweighted least squares to
+// the relative error (degree 3: 1.0e-4, degree 4: 2.8e-6, below the rounding of a weight to bf16, f16).
+// Exactly 0 at and below y = -127, where a masked place's -inf ends up.
 template <int DT>
-__device__ __forceinline__ bool any_nonfinite(unsigned w) {  // of the two 16-bit values
-  constexpr unsigned kExp = DT == COW_BF16 ? 0x7f807f80u : 0x7c007c00u;
-  const unsigned z = ~w & kExp;  // a half of zero: all exponent bits set
-  return ((z - 0x00010001u) & ~z & 0x80008000u) != 0;
+__device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, held in the low bits
+  float2 y = both(y2);
+  y2 = pair(fmaxf(y.x, -127.f), fmaxf(y.y, -127.f));
+  const uint64_t t = add2(y2, pair(kMagic, kMagic));
+  const uint64_t f = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f), y2);
+  uint64_t p;
+  if constexpr (DT == COW_BF16) {
+    p = fma2(f, pair(0.05500892922282219f, 0.05500892922282219f), pair(0.2422109693288803f, 0.2422109693288803f));
+    p = fma2(p, f, pair(0.6932829022407532f, 0.6932829022407532f));
+  } else {
+    p = fma2(f, pair(0.009582852944731712f, 0.009582852944731712f), pair(0.055906426161527634f, 0.055906426161527634f));
+    p = fma2(p, f, pair(0.24024099111557007f, 0.24024099111557007f));
+    p = fma2(p, f, pair(0.6931241750717163f, 0.6931241750717163f));
+  }
+  p = fma2(p, f, pair(1.f, 1.f));
+  const float2 r = both(p), n = both(t);
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+}
+
+// 0 * w + sum of two 16-bit values
+template <int DT>
+__device__ __forceinline__ unsigned zero_times(unsigned w, unsigned sum) {
+  unsigned r;
+  if constexpr (DT == COW_BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(sum));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(sum));
+  return r;
 }
 
 template <int DT, int DP>
@@ -358,6 +445,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   __shared__ Tile s_tile;
   __shared__ unsigned s_tmem;
   __shared__ int s_abort, s_bad;
+  __shared__ float s_most[2][2][kTcRows];
   const PromptLaunch& P = L.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = P.group, tile_tokens = kTcRows / group, kv_head = blockIdx.x % P.kv_heads;
@@ -365,10 +453,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   uint8_t* s_q = smem;                          // tiles A and B
   uint8_t* s_ring = smem + 2 * S::kTileBytes;
 
-  if (warp == 8) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     if (lane == 0) {
       s_abort = s_bad = 0;
       for (int i = 0; i < S::kSlots; ++i) {
@@ -378,14 +466,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
       mbar_init(&bars.q, 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars.s[i], 1);
-        mbar_init(&bars.p[i], 4);
+        mbar_init(&bars.p[i][0], 8);
+        mbar_init(&bars.p[i][1], 8);
         mbar_init(&bars.o[i], 1);
         mbar_init(&bars.look[i], 1);
-        mbar_init(&bars.looked[i], 2);
+        mbar_init(&bars.looked[i], 1);
       }
       mbar_init(&bars.drain, 1);
     }
-  } else if (warp == 10) {
+  } else if (warp == 18) {
     const Tile t = find_tile(P, 2 * tile_tokens, blockIdx.x / P.kv_heads);
     if (lane == 0) s_tile = t;
   }
@@ -396,6 +485,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   const Tile t = s_tile;
   volatile int* abort = &s_abort;
   auto wait = [&](uint64_t* bar, unsigned parity) {
+    if (mbar_wait(bar, parity, 4)) return true;
     if (*abort) return false;
     if (mbar_wait(bar, parity, kTcLimit)) return true;
     *abort = 1;
@@ -410,7 +500,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   const int masked_from = t.first / kTcKeys;  // key tiles from here on are not seen whole by every row
 
   if (t.count > 0) {
-    if (warp == 8 && lane == 0) {
+    if (warp == 16 && elect_one()) {
       // ---- loads
       mbar_arrive_expect_tx(&bars.q, (here_b > 0 ? 2 : 1) * S::kParts * 128 * group * tile_tokens);
       for (int x = 0; x < (here_b > 0 ? 2 : 1); ++x)
@@ -430,57 +520,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
       // nothing may still be on its way into shared memory when the block ends
       mbar_wait(&bars.q, 0, kTcLimit);
       for (int i = max(issued - S::kSlots, 0); i < issued; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, kTcLimit);
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 17 && elect_one()) {
       // ---- products
-      const int steps = (P.width + 15) / 16;
+      constexpr int kSteps = DP / 16;
       constexpr unsigned kType = DT == COW_BF16 ? 1u : 0u;
       const unsigned base = (1u << 4) | (kType << 7) | (kType << 10) | ((128u >> 4) << 24);
       // S: 128 x 128, both operands contiguous along the width; a negative scale negates Q
       const unsigned idesc_s = base | ((128u >> 3) << 17) | (P.scale_log2 < 0.f ? 1u << 13 : 0u);
       // O: 128 x width, values contiguous along the output's columns
-      const unsigned idesc_o = base | (1u << 16) | (static_cast<unsigned>(2 * steps) << 17);
+      const unsigned idesc_o = base | (1u << 16) | (static_cast<unsigned>(2 * kSteps) << 17);
+      const uint64_t desc_q = operand_at(smem_addr(s_q), 16), desc_ring = operand_at(smem_addr(s_ring), 16);
+      const uint64_t desc_v = operand_at(smem_addr(s_ring), S::kPartBytes);
       auto score = [&](int x, int j) {
-        const unsigned q = smem_addr(s_q) + x * S::kTileBytes, k = smem_addr(s_ring) + (2 * j % S::kSlots) * S::kTileBytes;
-        for (int i = 0; i < steps; ++i) {
-          const unsigned off = (i / 4) * S::kPartBytes + (i % 4) * 32;
-          tc_mma_ss(tmem + 128 * x, operand_at(q + off, 16), operand_at(k + off, 16), idesc_s, i > 0);
+        const uint64_t q = desc_q + x * (S::kTileBytes >> 4), k = desc_ring + (2 * j % S::kSlots) * (S::kTileBytes >> 4);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int off = ((i / 4) * S::kPartBytes + (i % 4) * 32) >> 4;
+          tc_mma_ss(tmem + 128 * x, q + off, k + off, idesc_s, i > 0);
         }
+        tc_commit(&bars.s[x]);
       };
-      auto output = [&](int x, int j) {
-        const unsigned v = smem_addr(s_ring) + ((2 * j + 1) % S::kSlots) * S::kTileBytes;
-        for (int i = 0; i < kTcKeys / 16; ++i)
-          tc_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * i, operand_at(v + 2048 * i, S::kPartBytes), idesc_o, j > 0 || i > 0);
+      auto output = [&](int x, int j, int h) {  // of each half of the tile's tokens, its half h
+        const uint64_t v = desc_v + ((2 * j + 1) % S::kSlots) * (S::kTileBytes >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          tc_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 64 * (i / 2) + 16 * h + 8 * (i % 2),
+                    v + (2048 >> 4) * (4 * (i / 2) + 2 * h + i % 2), idesc_o, j > 0 || h > 0 || i > 0);
       };
       auto full = [&](int i) { return wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1); };
+      // the tiles that the products of step j read; those of a masked tile's values are looked through
+      auto ready = [&](int j) {
+        if (j >= n) return true;
+        if (!full(2 * j + 1)) return false;
+        if (j >= masked_from) mbar_arrive(&bars.look[j - masked_from]);
+        return j + 1 >= n || full(2 * j + 2);
+      };
       bool ok = wait(&bars.q, 0) && full(0);
       if (ok) {
         tc_fence_after();
         score(0, 0);
-        tc_commit(&bars.s[0]);
-        if (n_b > 0) {
-          score(1, 0);
-          tc_commit(&bars.s[1]);
-        }
+        if (n_b > 0) score(1, 0);
         tc_commit(&bars.empty[0]);
+        ok = ready(0);
       }
       for (int j = 0; ok && j < n; ++j) {
-        ok = full(2 * j + 1);
-        if (ok && j >= masked_from) mbar_arrive(&bars.look[j - masked_from]);
-        ok = ok && (j + 1 >= n || full(2 * j + 2));
+        if (j >= masked_from) ok = wait(&bars.looked[j - masked_from], 0);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int nx = x ? n_b : n_a;
-          if (!ok || j >= nx) continue;
-          ok = wait(&bars.p[x], j & 1) && (j < masked_from || wait(&bars.looked[j - masked_from], 0));
-          if (!ok) continue;
-          tc_fence_after();
-          output(x, j);
-          if (j + 1 < nx) {
-            score(x, j + 1);
-            tc_commit(&bars.s[x]);
-          } else {
-            tc_commit(&bars.o[x]);
+          if (ok && j < nx) {
+            ok = wait(&bars.p[x][0], j & 1);
+            if (ok) {
+              tc_fence_after();
+              output(x, j, 0);
+              ok = wait(&bars.p[x][1], j & 1);
+            }
+            if (ok) {
+              tc_fence_after();
+              output(x, j, 1);
+              if (j + 1 < nx) score(x, j + 1);
+              else tc_commit(&bars.o[x]);
+            }
           }
+          if (x == 0) ok = ok && ready(j + 1);  // while B's softmax is at work
         }
         if (ok) {
           tc_commit(&bars.empty[(2 * j + 1) % S::kSlots]);
@@ -491,24 +593,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         tc_commit(&bars.drain);
         mbar_wait(&bars.drain, 0, kTcLimit);
       }
-    } else if (warp >= 10) {
+    } else if (warp == 18) {
       // ---- values of masked tiles
       for (int j = masked_from; j < n; ++j) {
         const int slot = (2 * j + 1) % S::kSlots;
         if (!__all_sync(kFull, wait(&bars.look[j - masked_from], 0) && wait(&bars.full[slot], ((2 * j + 1) / S::kSlots) & 1))) break;
         uint4* words = reinterpret_cast<uint4*>(s_ring + slot * S::kTileBytes);
-        constexpr int kEach = S::kTileBytes / 16 / 64;
-        bool bad = false;
+        constexpr int kEach = S::kTileBytes / 16 / 32;
+        unsigned sum = 0;  // of 0 times each value, by halves: NaN once one is not finite
 #pragma unroll 8
         for (int i = 0; i < kEach; ++i) {
-          const uint4 w = words[i * 64 + (warp - 10) * 32 + lane];
-          bad |= any_nonfinite<DT>(w.x) | any_nonfinite<DT>(w.y) | any_nonfinite<DT>(w.z) | any_nonfinite<DT>(w.w);
+          const uint4 w = words[i * 32 + lane];
+          sum = zero_times<DT>(w.x, zero_times<DT>(w.y, zero_times<DT>(w.z, zero_times<DT>(w.w, sum))));
         }
-        if (bad) {
+        if ((sum & 0x7fff7fffu) != 0) {
           constexpr unsigned kExp = DT == COW_BF16 ? 0x7f80u : 0x7c00u;
           s_bad = 1;
           for (int i = 0; i < kEach; ++i) {
-            unsigned* w = reinterpret_cast<unsigned*>(words + i * 64 + (warp - 10) * 32 + lane);
+            unsigned* w = reinterpret_cast<unsigned*>(words + i * 32 + lane);
             for (int u = 0; u < 4; ++u) {
               if ((w[u] & kExp) == kExp) w[u] &= 0xffff0000u;
               if (((w[u] >> 16) & kExp) == kExp) w[u] &= 0xffffu;
@@ -519,86 +621,107 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.looked[j - masked_from]);
       }
-    } else if (warp < 8) {
+    } else if (warp < 16) {
       // ---- softmax
-      const int x = warp >> 2;
+      const int x = warp >> 3, half = (warp >> 2) & 1;  // this thread's half of the keys
       const int nx = x ? n_b : n_a, here = x ? here_b : here_a;
       const int row = tid & 127, first = t.first + x * tile_tokens;
       const int query = first + row / group;  // its place in the sequence
       const unsigned lanes = tmem + (static_cast<unsigned>(warp & 3) << 21);  // this warp's 32 lanes
-      const unsigned at_s = lanes + 128 * x, at_o = lanes + 256 + 128 * x;
+      const unsigned at_s = lanes + 128 * x + 64 * half, at_o = lanes + 256 + 128 * x;
+      const int meet = 1 + 4 * x + (warp & 3);  // the barrier of the two warps that share 32 rows
       const float c = fabsf(P.scale_log2);
-      float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to
+      float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to, the same in both halves
       bool ok = true;
       for (int j = 0; j < nx; ++j) {
         ok = __all_sync(kFull, wait(&bars.s[x], j & 1));
         if (!ok) break;
         tc_fence_after();
-        unsigned s[128];
+        unsigned s[64];
         tc_load32(at_s, s);
         tc_load32(at_s + 32, s + 32);
-        tc_load32(at_s + 64, s + 64);
-        tc_load32(at_s + 96, s + 96);
         tc_wait_loads();
         if (j * kTcKeys + kTcKeys - 1 > first) {
-          const int seen = query - j * kTcKeys;
+          const int seen = query - j * kTcKeys - 64 * half;
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
+          for (int i = 0; i < 64; ++i)
             if (i > seen) s[i] = 0xff800000u;
         }
-        float big[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float big[4];
 #pragma unroll
-        for (int i = 0; i < 128; ++i) big[i & 3] = fmaxf(big[i & 3], __uint_as_float(s[i]));
-        const float now = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * c;
-        const bool grown = now > m + kLazy || m == -INFINITY;
-        if (__any_sync(kFull, grown)) {
-          const float next = grown ? fmaxf(now, m) : m;
-          const float a = grown && next != -INFINITY ? exp2_fast(m - next) : 1.f;
+        for (int i = 0; i < 4; ++i) big[i] = __uint_as_float(s[i]);
+#pragma unroll
+        for (int i = 4; i < 64; i += 2) {
+          float& b = big[(i / 2) & 3];
+          b = max3_nan(b, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        }
+        float now = max3_nan(max3_nan(big[0], big[1], big[2]), big[3], big[3]) * c;
+        if (any_of_two_warps(meet, !(now <= m + kLazy))) {  // NaN too
+          s_most[x][half][row] = now;
+          two_warps_meet(meet);
+          now = max3_nan(now, s_most[x][half ^ 1][row], m);
+          const bool grown = !(now <= m + kLazy);
+          float next = grown ? now : m;
+          if (next == INFINITY) next = __int_as_float(0x7fc00000);  // inf - inf: the row is NaN, as any that sees one
+          const float a = next == -INFINITY ? 1.f : exp2_fast(m - next);
           m = next;
           l *= a;
           if (j > 0) {
 #pragma unroll 1
-            for (int i = 0; i < P.width; i += 32) {
-              unsigned o[32];
-              tc_load32(at_o + i, o);
+            for (int i = 8 * half; i < DP; i += 16) {  // few registers: the scores wait in theirs
+              unsigned o[8];
+              tc_load8(at_o + i, o);
               tc_wait_loads();
 #pragma unroll
-              for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
-              tc_store32(at_o + i, o);
+              for (int u = 0; u < 8; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * a);
+              tc_store8(at_o + i, o);
             }
+            tc_wait_stores();
           }
+          two_warps_meet(meet);  // both have rescaled, and read the other's maximum
         }
         const float base = m == -INFINITY ? 0.f : m;  // all -inf so far: weights 0
-        float sum[2] = {0.f, 0.f};
+        const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          unsigned p[32];
+          unsigned p[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e0 = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * i]), c, -base));
-            const float e1 = exp2_fast(fmaf(__uint_as_float(s[64 * h + 2 * i + 1]), c, -base));
-            sum[0] += e0;
-            sum[1] += e1;
-            p[i] = pack2<DT>(e0, e1);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t y = fma2(pair(__uint_as_float(s[32 * h + 2 * i]), __uint_as_float(s[32 * h + 2 * i + 1])), c2, base2);
+            float2 e;
+            if (i % 8 < S::kPoly) {
+              e = exp2_poly<DT>(y);
+            } else {
+              e = both(y);
+              e.x = exp2_fast(e.x);
+              e.y = exp2_fast(e.y);
+            }
+            sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
+            p[i] = pack2<DT>(e.x, e.y);
           }
-          tc_store32(at_s + 32 * h, p);
+          tc_store16(at_s + 16 * h, p);
+          tc_wait_stores();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.p[x][h]);
         }
-        l += sum[0] + sum[1];
-        tc_wait_stores();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p[x]);
+        const float2 sums = both(add2(sum[0], sum[1]));
+        l += sums.x + sums.y;
       }
       if (nx > 0) {
         ok = __all_sync(kFull, ok && wait(&bars.o[x], 0));
         tc_fence_after();
+        s_most[x][half][row] = l;
+        two_warps_meet(meet);
+        l += s_most[x][half ^ 1][row];
         const bool store = row / group < here;
         const float inv = ok ? 1.f / l : __int_as_float(0x7fc00000);
         uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.out) +
                                               (static_cast<int64_t>(t.begin + query) * P.heads +
                                                static_cast<int64_t>(kv_head) * group + row % group) * P.width);
 #pragma unroll 1
-        for (int i = 0; i < P.width; i += 32) {
+        for (int i = 32 * half; i < DP; i += 64) {
           unsigned o[32];
           __syncwarp();
           tc_load32(at_o + i, o);
@@ -637,7 +760,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -691,9 +814,11 @@ int prompt_tc(const PromptLaunch& P, cudaStream_t stream) {
   // every sequence adds at most one tile that is not full
   const int64_t tiles = P.tokens / (2 * tile_tokens) + (P.sequences < P.tokens ? P.sequences : P.tokens);
   const unsigned blocks = static_cast<unsigned>(tiles * P.kv_heads);
-  if (P.dtype == COW_BF16)
-    return P.width <= 64 ? launch_tc<COW_BF16, 64>(L, blocks, stream) : launch_tc<COW_BF16, 128>(L, blocks, stream);
-  return P.width <= 64 ? launch_tc<COW_F16, 64>(L, blocks, stream) : launch_tc<COW_F16, 128>(L, blocks, stream);
+  const bool bf16 = P.dtype == COW_BF16;
+  if (P.width <= 32) return bf16 ? launch_tc<COW_BF16, 32>(L, blocks, stream) : launch_tc<COW_F16, 32>(L, blocks, stream);
+  if (P.width <= 64) return bf16 ? launch_tc<COW_BF16, 64>(L, blocks, stream) : launch_tc<COW_F16, 64>(L, blocks, stream);
+  if (P.width <= 96) return bf16 ? launch_tc<COW_BF16, 96>(L, blocks, stream) : launch_tc<COW_F16, 96>(L, blocks, stream);
+  return bf16 ? launch_tc<COW_BF16, 128>(L, blocks, stream) : launch_tc<COW_F16, 128>(L, blocks, stream);
 }
 
 template <int D>
