@@ -200,7 +200,7 @@ _SIGNATURES = {
     "cow_kv8_attend_workspace_bytes": (c_int64, [P, c_int32]),
     "cow_kv8_attend": (c_int32, [P, c_int32, P, c_int64, c_int64, c_int32, c_int32, ctypes.c_float, P, P, c_int64, P]),
     "cow_prompt_attention": (c_int32, [P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64,
-                                       c_int64, c_int32, c_int32, c_int32, c_int32, ctypes.c_float, P, P]),
+                                       c_int64, c_int32, c_int32, c_int32, c_int32, ctypes.c_float, P, P, P]),
     "cow_validate_workspace_bytes": (c_int64, [POINTER(CowPool), c_int32]),
     "cow_validate_layers": (c_int32, [POINTER(CowPool), c_int32, P, c_int64, P, P]),
 }

@@ -7,7 +7,7 @@
 // their rows.  Keys pass in tiles of 64; maximum, sum and output of the running softmax stay in
 // registers.  Tiles run in the order of their work, longest first, over all sequences
 // together: the tile at place l of its sequence reads l + 1 tiles' keys, so the tiles of place l
-// are one for each sequence that has more than l, and a block finds its own by a search
+// are one for each sequence that has more than l, and one is found by a search
 // over l with no table to build.
 
 #include <cuda.h>
@@ -25,6 +25,7 @@ struct PromptLaunch {
   void* out;
   const int32_t* starts;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
+  int32_t* status;  // may be null
   int32_t sequences, tokens, heads, kv_heads, group, width, dtype;
   float scale_log2;  // scale * log2(e)
 };
@@ -39,43 +40,67 @@ struct Tile {
   int begin, count, first;  // its sequence, and its first token in it; count 0: none left
 };
 
-// The x-th tile of all in the order of work, found by one warp.
-__device__ __forceinline__ Tile find_tile(const PromptLaunch& P, int tile_tokens, int x) {
-  const int lane = threadIdx.x & 31;
-  const int B = P.sequences;
-  // tiles whose place is >= h
-  auto above = [&](int h) {
+// Finds tiles by their place in the order of work; all members are one warp's.  A lane keeps the tile
+// counts of kHeld sequences; those beyond 32 * kHeld are read again at every look.
+struct TileFinder {
+  static constexpr int kHeld = 4;
+  int held[kHeld];
+  int most, all;
+
+  __device__ __forceinline__ int tiles_of(const PromptLaunch& P, int tile_tokens, int b) const {
+    return b < P.sequences ? (sequence_of(P, b).y + tile_tokens - 1) / tile_tokens : 0;
+  }
+  // tiles whose place in their sequence is >= h
+  __device__ __forceinline__ int above(const PromptLaunch& P, int tile_tokens, int h) const {
     int n = 0;
-    for (int b = lane; b < B; b += 32) n += max((sequence_of(P, b).y + tile_tokens - 1) / tile_tokens - h, 0);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) n += max(held[i] - h, 0);
+    for (int b = 32 * kHeld + (threadIdx.x & 31); b < P.sequences; b += 32) n += max(tiles_of(P, tile_tokens, b) - h, 0);
     return __reduce_add_sync(kFull, n);
-  };
-  int most = 0;
-  for (int b = lane; b < B; b += 32) most = max(most, (sequence_of(P, b).y + tile_tokens - 1) / tile_tokens);
-  most = __reduce_max_sync(kFull, most);
-  Tile t{0, 0, 0};
-  if (x >= above(0)) return t;
-  int lo = 0, hi = most;  // above(lo) > x >= above(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (above(mid) > x) lo = mid; else hi = mid;
   }
-  int rank = x - above(hi);  // among the sequences with more than lo tiles
-  for (int base = 0; base < B; base += 32) {
-    int2 seq = make_int2(0, 0);
-    if (base + lane < B) seq = sequence_of(P, base + lane);
-    const unsigned has = __ballot_sync(kFull, (seq.y + tile_tokens - 1) / tile_tokens > lo);
-    const int n = __popc(has);
-    if (rank < n) {
-      const int src = __fns(has, 0, rank + 1);
-      t.begin = __shfl_sync(kFull, seq.x, src);
-      t.count = __shfl_sync(kFull, seq.y, src);
-      t.first = lo * tile_tokens;
-      return t;
+  __device__ __forceinline__ void begin(const PromptLaunch& P, int tile_tokens) {
+    const int lane = threadIdx.x & 31;
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      held[i] = tiles_of(P, tile_tokens, 32 * i + lane);
+      most = max(most, held[i]);
     }
-    rank -= n;
+    for (int b = 32 * kHeld + lane; b < P.sequences; b += 32) most = max(most, tiles_of(P, tile_tokens, b));
+    most = __reduce_max_sync(kFull, most);
+    all = above(P, tile_tokens, 0);
   }
-  return t;
-}
+  // The x-th tile in the order of work; none (count 0) from `all` on.
+  __device__ __forceinline__ Tile find(const PromptLaunch& P, int tile_tokens, int x) const {
+    const int lane = threadIdx.x & 31;
+    Tile t{0, 0, 0};
+    if (x >= all) return t;
+    int lo = 0, hi = most;  // above(lo) > x >= above(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (above(P, tile_tokens, mid) > x) lo = mid; else hi = mid;
+    }
+    int rank = x - above(P, tile_tokens, hi);  // among the sequences with more than lo tiles
+    int b = -1;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const unsigned has = __ballot_sync(kFull, held[i] > lo);
+      if (b < 0 && rank < __popc(has)) b = 32 * i + __fns(has, 0, rank + 1);
+      rank -= __popc(has);
+    }
+    for (int base = 32 * kHeld; b < 0 && base < P.sequences; base += 32) {
+      const unsigned has = __ballot_sync(kFull, tiles_of(P, tile_tokens, base + lane) > lo);
+      if (rank < __popc(has)) b = base + __fns(has, 0, rank + 1);
+      rank -= __popc(has);
+    }
+    if (b < 0) return t;
+    const int2 seq = sequence_of(P, b);
+    t.begin = seq.x;
+    t.count = seq.y;
+    t.first = lo * tile_tokens;
+    return t;
+  }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -106,7 +131,9 @@ __global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_c
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int group = P.group, tile_tokens = kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
   if (tid < 32) {
-    const Tile t = find_tile(P, tile_tokens, blockIdx.x / P.kv_heads);
+    TileFinder finder;
+    finder.begin(P, tile_tokens);
+    const Tile t = finder.find(P, tile_tokens, blockIdx.x / P.kv_heads);
     if (tid == 0) s_tile = t;
   }
   __syncthreads();
@@ -229,13 +256,14 @@ __global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_c
 // 16-bit types: tcgen05
 // --------------------------------------------------------------------------
 //
-// A block has two tiles A and B of 128 rows against key tiles of 128 tokens, twenty warps:
+// A block, one to an SM, has two tiles A and B of 128 rows against key tiles of 128 tokens, twenty warps:
 //   warps 0-7, 8-15  softmax of A and of B: two threads to a row, 64 keys each, so that the row's scores
 //                    fit registers with four warps to a scheduler; the two meet once a key tile
 //   warp 16          one thread loads by TMA: the query tiles once, K and V tiles round a ring
 //   warp 17          one thread issues the products: S = Q K^T into tensor memory, and O += P V
 //                    with P read from tensor memory, where it takes the place of S
 //   warp 18          looks through the values of masked tiles (below)
+//   warp 19          finds the next tiles
 // While one tile's softmax runs, the tensor cores work on the other's O += P V and next S; S(j + 1) of a
 // tile is issued after O += P V (j) of it, so its arrival also says that O may be touched.
 // O lies in tensor memory for the whole pass.  It is rescaled only when a row's maximum has grown by more
@@ -248,12 +276,14 @@ __global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_c
 // other sequences) are looked through first, non-finite ones are taken out, and rows that do see
 // them have them added at the end.
 //
-// Every wait is bounded; one that gives up ends the block with NaN rows.
+// A block stays and takes tile after tile: loads and scores of the next begin under the end of the last.
+// Every wait is bounded; one that gives up sets a status bit and ends the block, its current rows NaN.
 
 constexpr int kTcThreads = 640;
 constexpr int kTcRows = 128;  // rows of a tile
 constexpr int kTcKeys = 128;  // tokens of a key tile
-constexpr int kTcLimit = 1 << 18;
+constexpr int kTcLimit = 1 << 18;                        // tries of the waits at a block's end
+constexpr unsigned long long kTcPatience = 2000000000ull;  // ns of the others
 constexpr float kLazy = 8.f;  // log2 of the growth of a maximum that is let pass
 
 template <int DP>  // width rounded up to 32s
@@ -272,8 +302,23 @@ struct TcLaunch {
 };
 
 struct TcBarriers {
-  uint64_t full[8], empty[8];
-  uint64_t q, s[2], p[2][2], o[2], look[2], looked[2], drain;  // look, looked: at most two tiles are masked
+  uint64_t full[8], empty[8];         // the ring
+  uint64_t tile_full[2], tile_empty[2];  // what to work on
+  uint64_t q_full, q_empty;
+  uint64_t s[2], p[2][2];             // scores are there; halves of the weights are
+  uint64_t o_full[2], o_empty[2];     // the output is complete; is read
+  uint64_t look[2], looked[2];        // a masked tile's values are there; are looked through (two such tiles at most)
+  uint64_t drain;
+};
+
+// What a block works on: two tiles of rows of one key head.
+struct TcTile {
+  int begin, count, first, kv_head;  // count 0: no more
+  int here_a, here_b;                // tokens
+  int n_a, n_b;                      // key tiles
+  int masked_from;                   // key tiles from here on are not seen whole by every row
+
+  __device__ __forceinline__ int n() const { return max(n_a, n_b); }
 };
 
 // Two warps (64 threads) at named barrier `id`: whether `yes` holds in any of their threads; a plain meeting.
@@ -287,6 +332,12 @@ __device__ __forceinline__ bool any_of_two_warps(int id, bool yes) {
   return any != 0;
 }
 __device__ __forceinline__ void two_warps_meet(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+
+__device__ __forceinline__ unsigned long long nanoseconds() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
 
 // One thread of a converged warp, known to the compiler to be one.
 __device__ __forceinline__ bool elect_one() {
@@ -442,97 +493,144 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   using S = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcBarriers bars;
-  __shared__ Tile s_tile;
+  __shared__ TcTile s_tiles[2];
+  __shared__ int s_bad[2];
   __shared__ unsigned s_tmem;
-  __shared__ int s_abort, s_bad;
+  __shared__ int s_abort;
   __shared__ float s_most[2][2][kTcRows];
   const PromptLaunch& P = L.p;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int group = P.group, tile_tokens = kTcRows / group, kv_head = blockIdx.x % P.kv_heads;
+  const int group = P.group, tile_tokens = kTcRows / group;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* s_q = smem;                          // tiles A and B
+  uint8_t* s_q = smem;  // tiles A and B
   uint8_t* s_ring = smem + 2 * S::kTileBytes;
 
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  } else if (warp == 17) {
-    if (lane == 0) {
-      s_abort = s_bad = 0;
-      for (int i = 0; i < S::kSlots; ++i) {
-        mbar_init(&bars.full[i], 1);
-        mbar_init(&bars.empty[i], 1);
-      }
-      mbar_init(&bars.q, 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars.s[i], 1);
-        mbar_init(&bars.p[i][0], 8);
-        mbar_init(&bars.p[i][1], 8);
-        mbar_init(&bars.o[i], 1);
-        mbar_init(&bars.look[i], 1);
-        mbar_init(&bars.looked[i], 1);
-      }
-      mbar_init(&bars.drain, 1);
+  } else if (warp == 17 && lane == 0) {
+    s_abort = 0;
+    for (int i = 0; i < S::kSlots; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.empty[i], 1);
     }
-  } else if (warp == 18) {
-    const Tile t = find_tile(P, 2 * tile_tokens, blockIdx.x / P.kv_heads);
-    if (lane == 0) s_tile = t;
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.tile_full[i], 1);
+      mbar_init(&bars.tile_empty[i], 19);  // loads, products, looking through, 16 softmax warps
+      mbar_init(&bars.s[i], 1);
+      mbar_init(&bars.p[i][0], 8);
+      mbar_init(&bars.p[i][1], 8);
+      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.o_empty[i], 8);
+      mbar_init(&bars.look[i], 1);
+      mbar_init(&bars.looked[i], 1);
+    }
+    mbar_init(&bars.drain, 1);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = s_tmem;
-  const Tile t = s_tile;
   volatile int* abort = &s_abort;
   auto wait = [&](uint64_t* bar, unsigned parity) {
     if (mbar_wait(bar, parity, 4)) return true;
-    if (*abort) return false;
-    if (mbar_wait(bar, parity, kTcLimit)) return true;
-    *abort = 1;
-    return false;
+    const unsigned long long since = nanoseconds();
+    while (!mbar_wait(bar, parity, 64)) {
+      if (*abort) return false;
+      if (nanoseconds() - since > kTcPatience) {
+        *abort = 1;
+        return false;
+      }
+    }
+    return true;
+  };
+  // the i-th of this block's tiles; false: none left, or a wait gave up
+  auto next_tile = [&](int i, TcTile& t) {
+    if (!wait(&bars.tile_full[i & 1], (i >> 1) & 1)) return false;
+    t = s_tiles[i & 1];
+    return t.count > 0;
   };
 
-  // tokens and key tiles of A and B
-  const int here_a = min(tile_tokens, t.count - t.first), here_b = max(min(tile_tokens, t.count - t.first - tile_tokens), 0);
-  const int n_a = (t.first + here_a + kTcKeys - 1) / kTcKeys;
-  const int n_b = here_b > 0 ? (t.first + tile_tokens + here_b + kTcKeys - 1) / kTcKeys : 0;
-  const int n = max(n_a, n_b);
-  const int masked_from = t.first / kTcKeys;  // key tiles from here on are not seen whole by every row
-
-  if (t.count > 0) {
-    if (warp == 16 && elect_one()) {
-      // ---- loads
-      mbar_arrive_expect_tx(&bars.q, (here_b > 0 ? 2 : 1) * S::kParts * 128 * group * tile_tokens);
-      for (int x = 0; x < (here_b > 0 ? 2 : 1); ++x)
-        for (int part = 0; part < S::kParts; ++part)
-          tma_load(s_q + x * S::kTileBytes + part * S::kPartBytes, &L.q, 64 * part, kv_head * group,
-                   t.begin + t.first + x * tile_tokens, &bars.q);
-      int issued = 0;
-      for (int i = 0; i < 2 * n; ++i) {  // K(0), V(0), K(1), ...
-        const int slot = i % S::kSlots;
-        if (i >= S::kSlots && !wait(&bars.empty[slot], (i / S::kSlots - 1) & 1)) break;
+  if (warp == 19) {
+    // ---- what to work on: tiles in the order of their work, back and forth over the blocks so that
+    // each gets large and small ones
+    TileFinder finder;
+    finder.begin(P, 2 * tile_tokens);
+    for (int i = 0;; ++i) {
+      const int w = i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const Tile f = finder.find(P, 2 * tile_tokens, w / P.kv_heads);
+      if (i >= 2 && !__all_sync(kFull, wait(&bars.tile_empty[i & 1], ((i >> 1) - 1) & 1))) break;
+      if (lane == 0) {
+        TcTile t;
+        t.begin = f.begin;
+        t.count = f.count;
+        t.first = f.first;
+        t.kv_head = w % P.kv_heads;
+        t.here_a = min(tile_tokens, f.count - f.first);
+        t.here_b = max(min(tile_tokens, f.count - f.first - tile_tokens), 0);
+        t.n_a = (f.first + t.here_a + kTcKeys - 1) / kTcKeys;
+        t.n_b = t.here_b > 0 ? (f.first + tile_tokens + t.here_b + kTcKeys - 1) / kTcKeys : 0;
+        t.masked_from = f.first / kTcKeys;
+        s_tiles[i & 1] = t;
+        s_bad[i & 1] = 0;
+        mbar_arrive(&bars.tile_full[i & 1]);
+      }
+      if (f.count == 0) break;
+    }
+  } else if (warp == 16 && elect_one()) {
+    // ---- loads
+    TcTile t;
+    int item = 0, tiles = 0;  // tiles of K and V, and of queries, so far
+    bool ok = true;
+    for (; ok && next_tile(tiles, t); ++tiles) {
+      auto load = [&](int i) {  // K(0), V(0), K(1), ...
+        const int slot = item % S::kSlots;
+        if (item >= S::kSlots && !wait(&bars.empty[slot], (item / S::kSlots - 1) & 1)) return false;
         mbar_arrive_expect_tx(&bars.full[slot], S::kTileBytes);
         for (int part = 0; part < S::kParts; ++part)
-          tma_load(s_ring + slot * S::kTileBytes + part * S::kPartBytes, i & 1 ? &L.v : &L.k, 64 * part, kv_head,
+          tma_load(s_ring + slot * S::kTileBytes + part * S::kPartBytes, i & 1 ? &L.v : &L.k, 64 * part, t.kv_head,
                    t.begin + (i >> 1) * kTcKeys, &bars.full[slot]);
-        issued = i + 1;
-      }
-      // nothing may still be on its way into shared memory when the block ends
-      mbar_wait(&bars.q, 0, kTcLimit);
-      for (int i = max(issued - S::kSlots, 0); i < issued; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, kTcLimit);
-    } else if (warp == 17 && elect_one()) {
-      // ---- products
-      constexpr int kSteps = DP / 16;
-      constexpr unsigned kType = DT == COW_BF16 ? 1u : 0u;
-      const unsigned base = (1u << 4) | (kType << 7) | (kType << 10) | ((128u >> 4) << 24);
-      // S: 128 x 128, both operands contiguous along the width; a negative scale negates Q
-      const unsigned idesc_s = base | ((128u >> 3) << 17) | (P.scale_log2 < 0.f ? 1u << 13 : 0u);
-      // O: 128 x width, values contiguous along the output's columns
-      const unsigned idesc_o = base | (1u << 16) | (static_cast<unsigned>(2 * kSteps) << 17);
-      const uint64_t desc_q = operand_at(smem_addr(s_q), 16), desc_ring = operand_at(smem_addr(s_ring), 16);
-      const uint64_t desc_v = operand_at(smem_addr(s_ring), S::kPartBytes);
+        ++item;
+        return true;
+      };
+      ok = load(0) && (tiles == 0 || wait(&bars.q_empty, (tiles - 1) & 1));
+      if (!ok) break;
+      const int both_tiles = t.here_b > 0 ? 2 : 1;
+      mbar_arrive_expect_tx(&bars.q_full, both_tiles * S::kParts * 128 * group * tile_tokens);
+      for (int x = 0; x < both_tiles; ++x)
+        for (int part = 0; part < S::kParts; ++part)
+          tma_load(s_q + x * S::kTileBytes + part * S::kPartBytes, &L.q, 64 * part, t.kv_head * group,
+                   t.begin + t.first + x * tile_tokens, &bars.q_full);
+      const int n = t.n();
+      for (int i = 1; ok && i < 2 * n; ++i) ok = load(i);
+      mbar_arrive(&bars.tile_empty[tiles & 1]);
+    }
+    // nothing may still be on its way into shared memory when the block ends
+    if (tiles > 0) mbar_wait(&bars.q_full, (tiles - 1) & 1, kTcLimit);
+    if (!ok) mbar_wait(&bars.q_full, tiles & 1, 4096);  // the tile that was broken off, if it got that far
+    for (int i = max(item - S::kSlots, 0); i < item; ++i) mbar_wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1, kTcLimit);
+  } else if (warp == 17 && elect_one()) {
+    // ---- products
+    constexpr int kSteps = DP / 16;
+    constexpr unsigned kType = DT == COW_BF16 ? 1u : 0u;
+    const unsigned base = (1u << 4) | (kType << 7) | (kType << 10) | ((128u >> 4) << 24);
+    // S: 128 x 128, both operands contiguous along the width; a negative scale negates Q
+    const unsigned idesc_s = base | ((128u >> 3) << 17) | (P.scale_log2 < 0.f ? 1u << 13 : 0u);
+    // O: 128 x width, values contiguous along the output's columns
+    const unsigned idesc_o = base | (1u << 16) | (static_cast<unsigned>(2 * kSteps) << 17);
+    const uint64_t desc_q = operand_at(smem_addr(s_q), 16), desc_ring = operand_at(smem_addr(s_ring), 16);
+    const uint64_t desc_v = operand_at(smem_addr(s_ring), S::kPartBytes);
+    TcTile t;
+    int item = 0;                                  // the tile's K(0) in the count of all K and V tiles
+    unsigned steps[2] = {0, 0}, done[2] = {0, 0};  // key tiles, and tiles of rows, of A and of B so far
+    unsigned looks[2] = {0, 0};
+    bool ok = true;
+    for (int tiles = 0; ok && next_tile(tiles, t); ++tiles) {
+      const int n = t.n();
       auto score = [&](int x, int j) {
-        const uint64_t q = desc_q + x * (S::kTileBytes >> 4), k = desc_ring + (2 * j % S::kSlots) * (S::kTileBytes >> 4);
+        const uint64_t q = desc_q + x * (S::kTileBytes >> 4), k = desc_ring + ((item + 2 * j) % S::kSlots) * (S::kTileBytes >> 4);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
           const int off = ((i / 4) * S::kPartBytes + (i % 4) * 32) >> 4;
@@ -541,101 +639,132 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         tc_commit(&bars.s[x]);
       };
       auto output = [&](int x, int j, int h) {  // of each half of the tile's tokens, its half h
-        const uint64_t v = desc_v + ((2 * j + 1) % S::kSlots) * (S::kTileBytes >> 4);
+        const uint64_t v = desc_v + ((item + 2 * j + 1) % S::kSlots) * (S::kTileBytes >> 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           tc_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 64 * (i / 2) + 16 * h + 8 * (i % 2),
                     v + (2048 >> 4) * (4 * (i / 2) + 2 * h + i % 2), idesc_o, j > 0 || h > 0 || i > 0);
       };
-      auto full = [&](int i) { return wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1); };
+      auto full = [&](int i) { return wait(&bars.full[(item + i) % S::kSlots], ((item + i) / S::kSlots) & 1); };
       // the tiles that the products of step j read; those of a masked tile's values are looked through
       auto ready = [&](int j) {
         if (j >= n) return true;
         if (!full(2 * j + 1)) return false;
-        if (j >= masked_from) mbar_arrive(&bars.look[j - masked_from]);
+        if (j >= t.masked_from) mbar_arrive(&bars.look[j - t.masked_from]);
         return j + 1 >= n || full(2 * j + 2);
       };
-      bool ok = wait(&bars.q, 0) && full(0);
+      ok = full(0) && wait(&bars.q_full, tiles & 1);
       if (ok) {
         tc_fence_after();
         score(0, 0);
-        if (n_b > 0) score(1, 0);
-        tc_commit(&bars.empty[0]);
+        if (t.n_b > 0) score(1, 0);
+        tc_commit(&bars.empty[item % S::kSlots]);
+        if (n == 1) tc_commit(&bars.q_empty);
         ok = ready(0);
       }
       for (int j = 0; ok && j < n; ++j) {
-        if (j >= masked_from) ok = wait(&bars.looked[j - masked_from], 0);
+        if (j >= t.masked_from) {
+          const int k = j - t.masked_from;
+          ok = wait(&bars.looked[k], looks[k] & 1);
+          ++looks[k];
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int nx = x ? n_b : n_a;
+          const int nx = x ? t.n_b : t.n_a;
           if (ok && j < nx) {
-            ok = wait(&bars.p[x][0], j & 1);
+            const unsigned phase = steps[x] & 1;
+            ++steps[x];
+            // the previous tile's output must have been read before the first product of this one's
+            ok = (j > 0 || done[x] == 0 || wait(&bars.o_empty[x], (done[x] - 1) & 1)) && wait(&bars.p[x][0], phase);
             if (ok) {
               tc_fence_after();
               output(x, j, 0);
-              ok = wait(&bars.p[x][1], j & 1);
+              ok = wait(&bars.p[x][1], phase);
             }
             if (ok) {
               tc_fence_after();
               output(x, j, 1);
-              if (j + 1 < nx) score(x, j + 1);
-              else tc_commit(&bars.o[x]);
+              if (j + 1 < nx) {
+                score(x, j + 1);
+              } else {
+                tc_commit(&bars.o_full[x]);
+                ++done[x];
+              }
             }
           }
           if (x == 0) ok = ok && ready(j + 1);  // while B's softmax is at work
         }
         if (ok) {
-          tc_commit(&bars.empty[(2 * j + 1) % S::kSlots]);
-          if (j + 1 < n) tc_commit(&bars.empty[(2 * j + 2) % S::kSlots]);
+          tc_commit(&bars.empty[(item + 2 * j + 1) % S::kSlots]);
+          if (j + 1 < n) tc_commit(&bars.empty[(item + 2 * j + 2) % S::kSlots]);
+          if (j + 2 == n) tc_commit(&bars.q_empty);  // the last scores are issued
         }
       }
-      if (!ok) {  // products in flight end before tensor memory is given back
-        tc_commit(&bars.drain);
-        mbar_wait(&bars.drain, 0, kTcLimit);
-      }
-    } else if (warp == 18) {
-      // ---- values of masked tiles
-      for (int j = masked_from; j < n; ++j) {
-        const int slot = (2 * j + 1) % S::kSlots;
-        if (!__all_sync(kFull, wait(&bars.look[j - masked_from], 0) && wait(&bars.full[slot], ((2 * j + 1) / S::kSlots) & 1))) break;
-        uint4* words = reinterpret_cast<uint4*>(s_ring + slot * S::kTileBytes);
+      item += 2 * n;
+      if (ok) mbar_arrive(&bars.tile_empty[tiles & 1]);
+    }
+    // products in flight end before tensor memory is given back
+    tc_commit(&bars.drain);
+    mbar_wait(&bars.drain, 0, kTcLimit);
+  } else if (warp == 18) {
+    // ---- values of masked tiles
+    TcTile t;
+    int item = 0;
+    unsigned looks[2] = {0, 0};
+    bool ok = true;
+    for (int tiles = 0; ok && __all_sync(kFull, next_tile(tiles, t)); ++tiles) {
+      const int n = t.n();
+      for (int j = t.masked_from; ok && j < n; ++j) {
+        const int k = j - t.masked_from, i = item + 2 * j + 1;
+        ok = __all_sync(kFull, wait(&bars.look[k], looks[k] & 1) && wait(&bars.full[i % S::kSlots], (i / S::kSlots) & 1));
+        if (!ok) break;
+        ++looks[k];
+        uint4* words = reinterpret_cast<uint4*>(s_ring + (i % S::kSlots) * S::kTileBytes);
         constexpr int kEach = S::kTileBytes / 16 / 32;
         unsigned sum = 0;  // of 0 times each value, by halves: NaN once one is not finite
 #pragma unroll 8
-        for (int i = 0; i < kEach; ++i) {
-          const uint4 w = words[i * 32 + lane];
+        for (int u = 0; u < kEach; ++u) {
+          const uint4 w = words[u * 32 + lane];
           sum = zero_times<DT>(w.x, zero_times<DT>(w.y, zero_times<DT>(w.z, zero_times<DT>(w.w, sum))));
         }
         if ((sum & 0x7fff7fffu) != 0) {
           constexpr unsigned kExp = DT == COW_BF16 ? 0x7f80u : 0x7c00u;
-          s_bad = 1;
-          for (int i = 0; i < kEach; ++i) {
-            unsigned* w = reinterpret_cast<unsigned*>(words + i * 32 + lane);
-            for (int u = 0; u < 4; ++u) {
-              if ((w[u] & kExp) == kExp) w[u] &= 0xffff0000u;
-              if (((w[u] >> 16) & kExp) == kExp) w[u] &= 0xffffu;
+          s_bad[tiles & 1] = 1;
+          for (int u = 0; u < kEach; ++u) {
+            unsigned* w = reinterpret_cast<unsigned*>(words + u * 32 + lane);
+            for (int y = 0; y < 4; ++y) {
+              if ((w[y] & kExp) == kExp) w[y] &= 0xffff0000u;
+              if (((w[y] >> 16) & kExp) == kExp) w[y] &= 0xffffu;
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.looked[j - masked_from]);
+        if (lane == 0) mbar_arrive(&bars.looked[k]);
       }
-    } else if (warp < 16) {
-      // ---- softmax
-      const int x = warp >> 3, half = (warp >> 2) & 1;  // this thread's half of the keys
-      const int nx = x ? n_b : n_a, here = x ? here_b : here_a;
-      const int row = tid & 127, first = t.first + x * tile_tokens;
-      const int query = first + row / group;  // its place in the sequence
-      const unsigned lanes = tmem + (static_cast<unsigned>(warp & 3) << 21);  // this warp's 32 lanes
-      const unsigned at_s = lanes + 128 * x + 64 * half, at_o = lanes + 256 + 128 * x;
-      const int meet = 1 + 4 * x + (warp & 3);  // the barrier of the two warps that share 32 rows
-      const float c = fabsf(P.scale_log2);
+      item += 2 * n;
+      if (ok && lane == 0) mbar_arrive(&bars.tile_empty[tiles & 1]);
+    }
+  } else if (warp < 16) {
+    // ---- softmax
+    const int x = warp >> 3, half = (warp >> 2) & 1;  // this thread's half of the keys
+    const int row = tid & 127, row_token = row / group;
+    const unsigned lanes = tmem + (static_cast<unsigned>(warp & 3) << 21);  // this warp's 32 lanes
+    const unsigned at_s = lanes + 128 * x + 64 * half, at_o = lanes + 256 + 128 * x;
+    const int meet = 1 + 4 * x + (warp & 3);  // the barrier of the two warps that share 32 rows
+    const float c = fabsf(P.scale_log2);
+    unsigned steps = 0, done = 0;
+    bool ok = true;
+    for (int tiles = 0; ok; ++tiles) {
+      // A wait that gave up is only remembered: both warps of a pair go on to their common end of the tile.
+      if (any_of_two_warps(meet, !wait(&bars.tile_full[tiles & 1], (tiles >> 1) & 1))) break;
+      const TcTile& t = s_tiles[tiles & 1];
+      if (t.count == 0) break;
+      const int nx = x ? t.n_b : t.n_a;
+      const int first = t.first + x * tile_tokens, query = first + row_token;  // its place in the sequence
       float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to, the same in both halves
-      bool ok = true;
-      for (int j = 0; j < nx; ++j) {
-        ok = __all_sync(kFull, wait(&bars.s[x], j & 1));
-        if (!ok) break;
+      for (int j = 0; j < nx; ++j, ++steps) {
+        ok = __all_sync(kFull, wait(&bars.s[x], steps & 1)) && ok;
         tc_fence_after();
         unsigned s[64];
         tc_load32(at_s, s);
@@ -710,25 +839,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         l += sums.x + sums.y;
       }
       if (nx > 0) {
-        ok = __all_sync(kFull, ok && wait(&bars.o[x], 0));
+        ok = wait(&bars.o_full[x], done & 1) && ok;
+        ++done;
         tc_fence_after();
         s_most[x][half][row] = l;
-        two_warps_meet(meet);
+        ok = !any_of_two_warps(meet, !ok);
         l += s_most[x][half ^ 1][row];
-        const bool store = row / group < here;
+        two_warps_meet(meet);  // the next tile writes there
+        const bool store = row_token < (x ? t.here_b : t.here_a);
         const float inv = ok ? 1.f / l : __int_as_float(0x7fc00000);
         uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.out) +
                                               (static_cast<int64_t>(t.begin + query) * P.heads +
-                                               static_cast<int64_t>(kv_head) * group + row % group) * P.width);
+                                               static_cast<int64_t>(t.kv_head) * group + row % group) * P.width);
 #pragma unroll 1
         for (int i = 32 * half; i < DP; i += 64) {
           unsigned o[32];
           __syncwarp();
           tc_load32(at_o + i, o);
           tc_wait_loads();
-          if (store && s_bad) {  // seen values that are not finite, taken out of the product above
-            for (int j = masked_from * kTcKeys; j <= query; ++j) {
-              const uint16_t* v = static_cast<const uint16_t*>(P.v) + (t.begin + j) * P.v_token + kv_head * P.v_head + i;
+          if (store && s_bad[tiles & 1]) {  // seen values that are not finite, taken out of the product above
+            for (int j = t.masked_from * kTcKeys; j <= query; ++j) {
+              const uint16_t* v = static_cast<const uint16_t*>(P.v) + (t.begin + j) * P.v_token + t.kv_head * P.v_head + i;
 #pragma unroll
               for (int u = 0; u < 32; ++u) {
                 if (i + u < P.width) {
@@ -753,7 +884,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
             }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.o_empty[x]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.tile_empty[tiles & 1]);
     }
   }
   __syncwarp();
@@ -761,6 +897,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (tid == 0 && s_abort && P.status) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -797,9 +934,10 @@ bool encode_rows(CUtensorMap* map, int dtype, const void* base, int64_t tokens, 
 
 template <int DT, int DP>
 int launch_tc(const TcLaunch& L, unsigned blocks, cudaStream_t stream) {
-  if (!resident_blocks(reinterpret_cast<const void*>(cow_prompt_tc_kernel<DT, DP>), kTcThreads, TcShape<DP>::kBytes))
-    return COW_ERR_CUDA;
-  cow_prompt_tc_kernel<DT, DP><<<blocks, kTcThreads, TcShape<DP>::kBytes, stream>>>(L);
+  const int resident = resident_blocks(reinterpret_cast<const void*>(cow_prompt_tc_kernel<DT, DP>), kTcThreads, TcShape<DP>::kBytes);
+  if (!resident) return COW_ERR_CUDA;
+  const unsigned grid = blocks < static_cast<unsigned>(resident) ? blocks : static_cast<unsigned>(resident);
+  cow_prompt_tc_kernel<DT, DP><<<grid, kTcThreads, TcShape<DP>::kBytes, stream>>>(L);
   return launch_status();
 }
 
@@ -850,7 +988,7 @@ int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_
                          const void* keys, int64_t key_token_stride, int64_t key_head_stride, const void* values,
                          int64_t value_token_stride, int64_t value_head_stride, const int32_t* starts,
                          int64_t sequences, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t width,
-                         int32_t dtype, float scale, void* out, void* stream) {
+                         int32_t dtype, float scale, void* out, int32_t* status, void* stream) {
   if (!valid_dtype(dtype) || sequences < 0 || tokens < 0 || kv_heads < 1 || heads < 1 || heads % kv_heads || width < 1)
     return COW_ERR_INVALID;
   if (width % 8 || width > 128 || heads / kv_heads > kMaxGroup || tokens >= (int64_t{1} << 30) ||
@@ -864,7 +1002,7 @@ int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_
       !rows_ok(values, value_token_stride, value_head_stride, dtype) || !starts || !out || !aligned16(out))
     return COW_ERR_INVALID;
   PromptLaunch P{queries, keys, values, out, starts, query_token_stride, query_head_stride, key_token_stride,
-                 key_head_stride, value_token_stride, value_head_stride, static_cast<int32_t>(sequences),
+                 key_head_stride, value_token_stride, value_head_stride, status, static_cast<int32_t>(sequences),
                  static_cast<int32_t>(tokens), heads, kv_heads, heads / kv_heads, width, dtype,
                  scale * 1.4426950408889634f};
   return dtype == COW_F32 ? prompt_f32(P, as_stream(stream)) : prompt_tc(P, as_stream(stream));

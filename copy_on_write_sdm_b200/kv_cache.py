@@ -77,6 +77,18 @@ def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
     return t.clone(memory_format=torch.contiguous_format), heads * width, width
 
 
+_PROMPT_STATUS: dict[int, torch.Tensor] = {}
+
+
+def prompt_attention_status(device: torch.device) -> torch.Tensor:
+    """The device's status word of ``prompt_attention``: 0, or ``_lib.ST_WAIT_TIMEOUT`` once a
+    wait inside the kernel gave up and left rows unwritten."""
+    word = _PROMPT_STATUS.get(device.index)
+    if word is None:
+        word = _PROMPT_STATUS[device.index] = torch.zeros((), dtype=torch.int32, device=device)
+    return word
+
+
 def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, starts: torch.Tensor, *,
                      scale: float | None = None) -> torch.Tensor:
     """Causal attention over packed prompts.
@@ -107,7 +119,7 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
         raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
     out = torch.empty((tokens, heads, width), dtype=q.dtype, device=device)
     _call(device, "cow_prompt_attention", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
-          code, width ** -0.5 if scale is None else float(scale), out.data_ptr())
+          code, width ** -0.5 if scale is None else float(scale), out.data_ptr(), prompt_attention_status(device).data_ptr())
     return out
 
 

@@ -633,12 +633,13 @@ int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries
  * in dtype; strides in elements, positive, rows contiguous and 16-byte aligned, out
  * contiguous.  width a multiple of 8 up to 128, heads a multiple of kv_heads
  * with at most 64 query heads to a key head.  Tokens outside every sequence
- * are not written. */
+ * are not written.  status (a device word, may be NULL) gets
+ * COW_ST_WAIT_TIMEOUT if a wait inside a block gave up; rows are then missing. */
 int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_t query_head_stride,
                          const void* keys, int64_t key_token_stride, int64_t key_head_stride, const void* values,
                          int64_t value_token_stride, int64_t value_head_stride, const int32_t* starts,
                          int64_t sequences, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t width,
-                         int32_t dtype, float scale, void* out, void* stream);
+                         int32_t dtype, float scale, void* out, int32_t* status, void* stream);
 
 /* materialize_dense (allocator.py:1004-1017): dense [banks,slots,width] in out_dtype. */
 int cow_materialize(const cow_pool* pool, void* out, int32_t out_dtype, void* stream);

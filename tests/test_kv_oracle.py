@@ -89,7 +89,7 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
 
     def prompt(width=32, heads=4, kv_heads=2, dtype=0, q=base, stride=128, out=base):
         return lib.cow_prompt_attention(q, stride, 32, base, 64, 32, base, 64, 32, base, 1, 8, heads, kv_heads, width, dtype,
-                                        1.0, out, None)
+                                        1.0, out, None, None)
     assert prompt(q=None) == _lib.ERR_INVALID
     assert prompt(out=None) == _lib.ERR_INVALID
     assert prompt(stride=126) == _lib.ERR_INVALID
