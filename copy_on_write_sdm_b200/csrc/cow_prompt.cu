@@ -646,12 +646,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
                     v + (2048 >> 4) * (4 * (i / 2) + 2 * h + i % 2), idesc_o, j > 0 || h > 0 || i > 0);
       };
       auto full = [&](int i) { return wait(&bars.full[(item + i) % S::kSlots], ((item + i) / S::kSlots) & 1); };
-      // the tiles that the products of step j read; those of a masked tile's values are looked through
-      auto ready = [&](int j) {
+      // V(j) is there; a masked tile's values are looked through
+      auto values = [&](int j) {
         if (j >= n) return true;
         if (!full(2 * j + 1)) return false;
         if (j >= t.masked_from) mbar_arrive(&bars.look[j - t.masked_from]);
-        return j + 1 >= n || full(2 * j + 2);
+        return true;
       };
       ok = full(0) && wait(&bars.q_full, tiles & 1);
       if (ok) {
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         if (t.n_b > 0) score(1, 0);
         tc_commit(&bars.empty[item % S::kSlots]);
         if (n == 1) tc_commit(&bars.q_empty);
-        ok = ready(0);
+        ok = values(0) && (n == 1 || full(2));
       }
       for (int j = 0; ok && j < n; ++j) {
         if (j >= t.masked_from) {
@@ -692,8 +692,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
               }
             }
           }
-          if (x == 0) ok = ok && ready(j + 1);  // while B's softmax is at work
+          if (x == 0) ok = ok && values(j + 1);  // while B's softmax is at work
         }
+        ok = ok && (j + 2 >= n || full(2 * j + 4));  // K(j + 2), while A's is
         if (ok) {
           tc_commit(&bars.empty[(item + 2 * j + 1) % S::kSlots]);
           if (j + 1 < n) tc_commit(&bars.empty[(item + 2 * j + 2) % S::kSlots]);
