@@ -39,20 +39,13 @@ _STATUS_TEXT = [
 ]
 
 
-def _on_device(device: torch.device):
-    """The device made current for a call, where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return None
-    return torch.cuda.device(device)
-
-
 def _call(device: torch.device, what: str, *args) -> None:
+    """One entry point on the device's current stream, the device made current where it is not."""
     fn = getattr(_lib.load(), what)
-    guard = _on_device(device)
-    if guard is None:
+    if device.index == torch.cuda.current_device():
         rc = fn(*args, _lib.stream_of(device))
     else:
-        with guard:
+        with torch.cuda.device(device):
             rc = fn(*args, _lib.stream_of(device))
     if rc:
         _lib.check(rc, what)
@@ -117,7 +110,7 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
         raise ValueError("queries, keys, values and starts must be on one device")
     if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
-    out = torch.empty((tokens, heads, width), dtype=q.dtype, device=device)
+    out = q.new_empty((tokens, heads, width))
     _call(device, "cow_prompt_attention", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
           code, width ** -0.5 if scale is None else float(scale), out.data_ptr(), prompt_attention_status(device).data_ptr())
     return out
@@ -176,7 +169,6 @@ class PagedKVCache:
     status_word: torch.Tensor    # int32
     ticket: torch.Tensor         # int32
     _epoch: list = field(default_factory=lambda: [0], repr=False)
-    _own: dict = field(default_factory=dict, repr=False, init=False)
 
     @classmethod
     def allocate(cls, *, requests: int, pages: int, kv_heads: int, head_width: int, max_blocks: int, layers: int = 1,
@@ -207,35 +199,18 @@ class PagedKVCache:
             lengths=zeros(requests), free_pages=torch.arange(pages, dtype=torch.int32, device=device),
             free_count=torch.tensor(pages, dtype=torch.int32, device=device), status_word=zeros(), ticket=zeros())
 
-    # ---- sizes
-
-    @property
-    def device(self) -> torch.device:
-        return self.lengths.device
-
-    @property
-    def requests(self) -> int:
-        return self.lengths.shape[0]
-
-    @property
-    def layers(self) -> int:
-        return self.key_pages.shape[0]
-
-    @property
-    def pages(self) -> int:
-        return self.key_pages.shape[1]
-
-    @property
-    def kv_heads(self) -> int:
-        return self.key_pages.shape[2]
-
-    @property
-    def head_width(self) -> int:
-        return self.key_pages.shape[4]
-
-    @property
-    def max_blocks(self) -> int:
-        return self.block_tables.shape[1]
+    def __post_init__(self) -> None:
+        # The tensors are fixed for this object's life: sizes and the C descriptor are taken once.
+        layers, pages, kv_heads, _, width = self.key_pages.shape
+        requests, max_blocks = self.block_tables.shape
+        desc = _lib.CowKVPages(
+            *(t.data_ptr() for t in (self.key_pages, self.value_pages, self.key_scales, self.value_scales, self.block_tables,
+                                     self.lengths, self.free_pages, self.free_count, self.status_word, self.ticket)),
+            requests, max_blocks, pages, layers, kv_heads, width)
+        for name, value in (("device", self.lengths.device), ("requests", requests), ("layers", layers), ("pages", pages),
+                            ("kv_heads", kv_heads), ("head_width", width), ("max_blocks", max_blocks), ("_desc", desc),
+                            ("_at", ctypes.addressof(desc)), ("_workspaces", {})):
+            object.__setattr__(self, name, value)
 
     def storage_bytes(self) -> dict[str, int]:
         """Bytes reserved for codes and scales, and for tables and stack."""
@@ -243,19 +218,6 @@ class PagedKVCache:
         meta = (self.block_tables, self.lengths, self.free_pages, self.free_count, self.status_word, self.ticket)
         return {"kv_pages": sum(t.numel() * t.element_size() for t in pools),
                 "kv_metadata": sum(t.numel() * t.element_size() for t in meta)}
-
-    def _desc(self) -> int:
-        """Address of the C descriptor; the tensors it points to are fixed for this object's life."""
-        at = self._own.get("at")
-        if at is None:
-            desc = _lib.CowKVPages(
-                *(t.data_ptr() for t in (self.key_pages, self.value_pages, self.key_scales, self.value_scales,
-                                         self.block_tables, self.lengths, self.free_pages, self.free_count,
-                                         self.status_word, self.ticket)),
-                self.requests, self.max_blocks, self.pages, self.layers, self.kv_heads, self.head_width)
-            self._own["desc"] = desc
-            at = self._own["at"] = ctypes.addressof(desc)
-        return at
 
     # ---- operators
 
@@ -273,13 +235,15 @@ class PagedKVCache:
         if targets.dtype != torch.int32 or targets.ndim != 1 or targets.shape[0] != self.requests \
                 or targets.device != self.device or not targets.is_contiguous():
             raise ValueError("targets must be a contiguous int32 vector [requests] on the cache's device")
-        words = _lib.load().cow_pages_plan_words(self.requests, int(tokens))
-        if words < 0:
+        tokens = int(tokens)
+        if not 0 <= tokens < 1 << 31:
             raise ValueError("the number of new tokens is invalid")
+        requests = self.requests
+        words = 4 + 4 * min(tokens, tokens // PAGE_TOKENS + 2 * requests) + requests + 1 + 2 * tokens
         self._epoch[0] += 1
-        plan = PagePlan(self, self._epoch[0], int(tokens), torch.empty(words, dtype=torch.int32, device=self.device))
-        _call(self.device, "cow_pages_resize", self._desc(), targets.data_ptr(), plan.tokens, plan.buffer.data_ptr(), words)
-        return plan
+        buffer = targets.new_empty(words)
+        _call(self.device, "cow_pages_resize", self._at, targets.data_ptr(), tokens, buffer.data_ptr(), words)
+        return PagePlan(self, self._epoch[0], tokens, buffer)
 
     def store(self, keys: torch.Tensor, values: torch.Tensor, plan: PagePlan, *, layer: int = 0) -> None:
         """Quantise the plan's new tokens' ``keys`` and ``values`` ``[tokens, kv_heads, head_width]`` into ``layer``.
@@ -300,7 +264,7 @@ class PagedKVCache:
         (k, k0, k1), (v, v0, v1) = _rows(keys, "keys"), _rows(values, "values")
         if k.device != self.device or v.device != self.device:
             raise ValueError("keys and values must be on the cache's device")
-        _call(self.device, "cow_kv8_store", self._desc(), layer, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, _lib.dtype_code(k.dtype), plan.buffer.data_ptr(), plan.tokens)
+        _call(self.device, "cow_kv8_store", self._at, layer, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, _lib.dtype_code(k.dtype), plan.buffer.data_ptr(), plan.tokens)
 
     def read(self, slots: torch.Tensor, *, layer: int = 0, dtype: torch.dtype = torch.bfloat16):
         """Keys and values ``[slots, kv_heads, head_width]`` that the cache holds at ``slots`` (int32; zeros for -1)."""
@@ -309,9 +273,9 @@ class PagedKVCache:
         if not 0 <= layer < self.layers:
             raise ValueError("the K/V cache has no such layer")
         code = _lib.dtype_code(dtype)
-        out = torch.empty((2, slots.shape[0], self.kv_heads, self.head_width), dtype=dtype, device=self.device)
-        keys, values = out[0], out[1]
-        _call(self.device, "cow_kv8_read", self._desc(), layer, slots.data_ptr(), slots.shape[0], keys.data_ptr(),
+        shape = (slots.shape[0], self.kv_heads, self.head_width)
+        keys, values = slots.new_empty(shape, dtype=dtype), slots.new_empty(shape, dtype=dtype)
+        _call(self.device, "cow_kv8_read", self._at, layer, slots.data_ptr(), slots.shape[0], keys.data_ptr(),
               values.data_ptr(), code)
         return keys, values
 
@@ -323,8 +287,8 @@ class PagedKVCache:
         sqrt(head_width) by default; zeros for a request without tokens.  Calls that may overlap
         on the GPU need a ``workspace`` each (``new_workspace``).
         """
-        if queries.ndim != 3 or queries.shape[0] != self.requests or queries.shape[2] != self.head_width \
-                or queries.shape[1] < 1 or queries.shape[1] % self.kv_heads:
+        shape = queries.shape
+        if len(shape) != 3 or shape[0] != self.requests or shape[2] != self.head_width or shape[1] < 1 or shape[1] % self.kv_heads:
             raise ValueError("attend takes queries [requests, heads, head_width], heads a multiple of kv_heads")
         if not 0 <= layer < self.layers:
             raise ValueError("the K/V cache has no such layer")
@@ -332,20 +296,20 @@ class PagedKVCache:
         q, q0, q1 = _rows(queries, "queries")
         if q.device != self.device:
             raise ValueError("queries must be on the cache's device")
-        heads = q.shape[1]
+        heads = shape[1]
         if workspace is None:
-            workspace = self._own.get(heads)
+            workspace = self._workspaces.get(heads)
             if workspace is None:
-                workspace = self._own[heads] = self.new_workspace(heads)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _call(self.device, "cow_kv8_attend", self._desc(), layer, q.data_ptr(), q0, q1, code, heads,
+                workspace = self._workspaces[heads] = self.new_workspace(heads)
+        out = q.new_empty(queries.shape)
+        _call(self.device, "cow_kv8_attend", self._at, layer, q.data_ptr(), q0, q1, code, heads,
               self.head_width ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),
               workspace.numel())
         return out
 
     def new_workspace(self, heads: int) -> torch.Tensor:
         """A zero-filled workspace of ``attend`` for ``heads`` query heads."""
-        need = _lib.load().cow_kv8_attend_workspace_bytes(self._desc(), heads)
+        need = _lib.load().cow_kv8_attend_workspace_bytes(self._at, heads)
         if need < 0:
             raise ValueError("heads must be a multiple of kv_heads")
         return torch.zeros(need, dtype=torch.uint8, device=self.device)
