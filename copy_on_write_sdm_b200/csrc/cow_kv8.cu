@@ -6,7 +6,9 @@
 // is exact before its one rounding, and when a later token of the page needs a larger scale,
 // the codes already there move to it exactly (but for those that become subnormal).
 // Keys lie [token][width]; values lie transposed, [width][token], so that one lane's 16-byte
-// word of either is the operand of a matrix instruction without any exchange.
+// word of either is the operand of a matrix instruction without any exchange.  In rows of 128 keys' bytes
+// the two halves of odd tokens are exchanged: lanes that read the same half of neighbouring rows
+// then meet all banks of shared memory.
 
 #include <cuda_fp8.h>
 
@@ -47,6 +49,12 @@ __device__ __forceinline__ float2 decode2(unsigned codes) {  // the two low byte
 __device__ __forceinline__ unsigned recode4(unsigned codes, float ratio) {
   const float2 a = decode2(codes), b = decode2(codes >> 16);
   return encode4(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
+}
+
+// Byte `d` of token t's row in a page's keys.
+template <int D>
+__device__ __forceinline__ int key_at(int t, int d) {
+  return t * D + (D == 128 ? d ^ ((t & 1) << 6) : d);
 }
 
 // 16 bytes of a tensor as floats
@@ -182,7 +190,7 @@ __global__ void __launch_bounds__(kStoreThreads) cow_kv8_store_kernel(const __gr
       if (v < tokens * kVecs) {
         float x[E];
         Vec16<DT>::get(w[i], x);
-        unsigned* out = reinterpret_cast<unsigned*>(dst + offset * D + v * E);
+        unsigned* out = reinterpret_cast<unsigned*>(dst + key_at<D>(offset + v / kVecs, v % kVecs * E));
 #pragma unroll
         for (int j = 0; j < E; j += 4) out[j / 4] = encode4(x[j] * inv, x[j + 1] * inv, x[j + 2] * inv, x[j + 3] * inv);
       }
@@ -301,7 +309,8 @@ __global__ void __launch_bounds__(kStoreThreads) cow_kv8_read_kernel(const __gri
         if (ok) {
           scale = P.scales[which][tile];
           codes = which ? *reinterpret_cast<const unsigned*>(&s_codes[i][4 * lane])
-                        : *reinterpret_cast<const unsigned*>(P.codes[0] + tile * (kPage * D) + (slot % kPage) * D + 4 * lane);
+                        : *reinterpret_cast<const unsigned*>(P.codes[0] + tile * (kPage * D) +
+                                                         (D == 128 ? key_at<128>(slot % kPage, 4 * lane) : (slot % kPage) * D + 4 * lane));
         }
         const float2 a = decode2(codes), b = decode2(codes >> 16);
         st4_rt(P.out[which], row * D + 4 * lane, make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale), P.dtype);
@@ -317,12 +326,16 @@ __global__ void __launch_bounds__(kStoreThreads) cow_kv8_read_kernel(const __gri
 // One query token per request, s_j = scale * ks * (q . k_j), o = sum_j softmax(s)_j vs v_j with
 // the code's k_j, v_j and the page's ks, vs.  Bound: memory, 2 * width bytes for each cached token
 // and key head, everything else is small.  So:
-// * the pages of all requests and heads form one list, cut into equal runs, one for each
-//   resident block, whatever the requests' lengths; a (request, head) pair that several blocks share
-//   is joined, in the order of its pages, by the block that finishes last;
-// * within a run a warp takes every fourth page; its K and V codes come by 16-byte asynchronous
-//   copies, the next page's keys while this page's values are used, and every lane reads back only
-//   what it copied itself, so nothing waits for another lane;
+// * the pages of all (request, head) pairs form one list, cut into units whatever the requests' lengths:
+//   a large one for each resident warp, then small ones taken as warps get free (SMs reach between 80 % and
+//   125 % of the mean rate here, so equal shares alone would wait for the slowest).  A pair inside one unit
+//   is answered from registers; parts of a pair go to global memory and a second kernel joins them, in the
+//   order of their pages.  (Joined by whichever warp came last instead, each join waited behind the
+//   queues of page loads for 10 us, a sixth of the whole time.)
+// * where no request has more than kAlignedPages and there are blocks for all pairs, each pair gets a block
+//   of its own instead and its warps' parts meet in shared memory;
+// * a page's K and its V come by one bulk copy each into the warp's own shared memory, the next page's keys
+//   while this page's values are used, on into the next pair; no warp waits for another;
 // * e4m3 is exact in f16, so both products run on m16n8k16 with f16 operands and f32 sums: pages are
 //   the 16-row operand (tokens, then width), the group's query heads the 8 columns, eight heads
 //   to a block.  The tcgen05 form would need the codes widened in shared memory first; here they
@@ -336,6 +349,12 @@ __global__ void __launch_bounds__(kStoreThreads) cow_kv8_read_kernel(const __gri
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = 32 * kAttendWarps;
 constexpr int kAttendHeads = 8;   // query heads of one block: the matrix instruction's columns
+constexpr int kJoin = 8;            // parts a warp of the second kernel reads at once
+// Threads of a block of the second kernel: few pairs have many parts each, and many pairs are best all at once
+// (32 pairs of 180 parts: 19 us with 128 threads; 512 pairs of 4: 16 us with 256).
+constexpr int kJoinFewPairs = 148, kJoinThreadsFew = 512, kJoinThreadsMany = 128;
+constexpr int kJoinColumns = 148 * 4;
+constexpr int kAlignedPages = 16;  // four pages a warp: less than a join through global memory takes
 constexpr float kProbShift = 8.f;  // probabilities are held times 2^8: more of f16's range below the largest
 
 struct AttendLaunch {
@@ -347,11 +366,13 @@ struct AttendLaunch {
   const int32_t* lengths;
   const char* q;
   char* out;
-  float* partials;  // [2 * blocks][8 * (width + 2)]
-  unsigned* arrived;  // [requests * pairs]
+  float* parts;       // [2 * units][rows of the group's heads (width, padded by 4): output, then maximum and sum]
+  unsigned* taken;    // [2] units taken, warps done: zero between calls
   int32_t* status;
   int64_t q_request_stride, q_head_stride;  // elements
   int64_t max_blocks;
+  int64_t slots;  // 2 * units that fit
+  int32_t warps;  // of the first kernel
   int32_t requests, kv_heads, heads, group, chunks, pages, dtype;
   float scale_log2;  // scale * log2(e)
 };
@@ -390,18 +411,6 @@ __device__ __forceinline__ unsigned pack_rest2(float a, float b, unsigned packed
   return pack_half2(a - h.x, b - h.y);
 }
 
-__device__ __forceinline__ void copy16(unsigned smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void copy8(unsigned smem, const void* gmem) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Lane (g = lane / 4, c = lane % 4) of a warp holds of a 64-token page, for the four 16-row steps s:
 //   keys:   tokens 16 (g/2) + 4 s + g%2 and that + 2 (rows g and g + 8 of step s), of each the 16 bytes
 //           64 h + 16 c of every whole 64-byte part h of the row and 8 bytes 64 H + 8 c of a last half one;
@@ -414,191 +423,391 @@ struct PageShape {
   static constexpr int kWhole = D / 64;                 // 64-byte parts of a key row
   static constexpr int kHalf = (D % 64) / 32;           // a last 32-byte part
   static constexpr int kKeySteps = D / 16;              // k16 steps of q . k
-  static constexpr int kValueRows = D / 8;              // value rows per lane
   static constexpr int kBytes = kPage * D;
 };
 
-template <int D>
-__device__ __forceinline__ void copy_keys(unsigned smem, const uint8_t* tile, int lane) {
-  using S = PageShape<D>;
-  const int g = lane >> 2, c = lane & 3;
-  const uint8_t* src = tile + ((g >> 1) * 16 + (g & 1)) * D;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {  // r = 2 s + half
-    const uint8_t* row = src + 2 * r * D;
-#pragma unroll
-    for (int h = 0; h < S::kWhole; ++h) copy16(smem + ((r * S::kWhole + h) * 32 + lane) * 16, row + 64 * h + 16 * c);
-    if constexpr (S::kHalf)
-      copy8(smem + S::kWhole * 64 * kPage + (r * 32 + lane) * 8, row + 64 * S::kWhole + 8 * c);
+// Pages of request b; the pages before each request (prefix [requests + 1] in shared memory), all of them
+// and the most of one request, by a block of kThreads.
+__device__ __forceinline__ int pages_of(const AttendLaunch& P, int b) {
+  return (min(max(P.lengths[b], 0), static_cast<int>(P.max_blocks) * kPage) + kPage - 1) / kPage;
+}
+template <int kThreads>
+__device__ __forceinline__ int2 scan_pages(const AttendLaunch& P, int* prefix, int2* s_scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = P.requests, per = (R + kThreads - 1) / kThreads;
+  int sum = 0, longest = 0;
+  for (int b = tid * per; b < min(R, (tid + 1) * per); ++b) {
+    const int n = pages_of(P, b);
+    sum += n;
+    longest = max(longest, n);
   }
-}
-template <int D>
-__device__ __forceinline__ void copy_values(unsigned smem, const uint8_t* tile, int lane) {
-  const int g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int i = 0; i < PageShape<D>::kValueRows; ++i) copy16(smem + (i * 32 + lane) * 16, tile + (8 * i + g) * kPage + 16 * c);
-}
-
-struct Run {  // the part of one (request, head chunk)'s pages that a block has
-  int request, pair, first, last, pages;  // pages first..last-1 of `pages`
-};
-
-template <int D, bool kSplit>
-__global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __grid_constant__ AttendLaunch P) {
-  using S = PageShape<D>;
-  constexpr int kRow = D + 2;  // a partial's row: output, maximum, sum
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-  uint8_t* s_keys = smem + warp * 2 * S::kBytes;
-  uint8_t* s_values = s_keys + S::kBytes;
-  int* s_prefix = reinterpret_cast<int*>(smem + kAttendWarps * 2 * S::kBytes);  // [requests + 1] pages before
-  __shared__ int s_scan[kAttendWarps];
-  __shared__ unsigned s_last;
-  const int R = P.requests, pairs = P.kv_heads * P.chunks, G = gridDim.x;
-
-  // pages of each request, and before it
-  const int per = (R + kAttendThreads - 1) / kAttendThreads;
-  const int most = static_cast<int>(P.max_blocks) * kPage;
-  int sum = 0;
-  for (int b = tid * per; b < min(R, (tid + 1) * per); ++b)
-    sum += (min(max(P.lengths[b], 0), most) + kPage - 1) / kPage;
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(kFull, inc, o);
     if (lane >= o) inc += x;
   }
-  if (lane == 31) s_scan[warp] = inc;
+  longest = __reduce_max_sync(kFull, longest);
+  if (lane == 31) s_scan[warp] = make_int2(inc, longest);
   __syncthreads();
   int at = inc - sum, all = 0;
-  for (int w = 0; w < kAttendWarps; ++w) {
-    if (w < warp) at += s_scan[w];
-    all += s_scan[w];
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) at += s_scan[w].x;
+    all += s_scan[w].x;
+    longest = max(longest, s_scan[w].y);
   }
   for (int b = tid * per; b < min(R, (tid + 1) * per); ++b) {
-    s_prefix[b] = at;
-    at += (min(max(P.lengths[b], 0), most) + kPage - 1) / kPage;
+    prefix[b] = at;
+    at += pages_of(P, b);
   }
-  if (tid == 0) s_prefix[R] = all;
+  if (tid == 0) prefix[R] = all;
   __syncthreads();
+  return make_int2(all, longest);
+}
+
+// A place in the list of pages: pair `pair` of request `b`, page p of np.
+struct Place {
+  int b, pair, p, np;
+};
+
+__device__ __forceinline__ Place place_of(const int* prefix, int requests, int pairs, int x) {
+  int lo = 0, hi = requests;  // the last request that begins at or before x: not an empty one
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] * pairs <= x) lo = mid; else hi = mid;
+  }
+  const int np = prefix[lo + 1] - prefix[lo];
+  const int at = x - prefix[lo] * pairs;
+  return Place{lo, at / np, at % np, np};
+}
+__device__ __forceinline__ void store_out(const AttendLaunch& P, int64_t at, float y) {
+  if (P.dtype == COW_F32) reinterpret_cast<float*>(P.out)[at] = y;
+  else if (P.dtype == COW_BF16) reinterpret_cast<__nv_bfloat16*>(P.out)[at] = __float2bfloat16_rn(y);
+  else reinterpret_cast<__half*>(P.out)[at] = __float2half_rn(y);
+}
+
+// The list cut into units: `warps` of `first` pages, then of `rest` pages.
+struct Units {
+  int total, first, rest, warps;
+  __device__ __forceinline__ int begin(int u) const {
+    return static_cast<int>(min(u < warps ? static_cast<int64_t>(u) * first : static_cast<int64_t>(warps) * first + static_cast<int64_t>(u - warps) * rest,
+                                static_cast<int64_t>(total)));
+  }
+  // The first units get 3/4 of the pages, the others eighths of a warp's share; not more units than the
+  // workspace holds parts for.
+  static __device__ __forceinline__ Units make(int total, int warps, int64_t slots) {
+    const int share = total / warps, first = max(share / 4 * 3 + share % 4 * 3 / 4, 1);
+    int rest = max((share + 8) / 8, 2);
+    const int room = static_cast<int>(slots / 2) - warps - 1, left = max(total - first * warps, 0);
+    if (left > static_cast<int64_t>(rest) * room) rest = left / room + 1;
+    return Units{total, first, rest, warps};
+  }
+  __device__ __forceinline__ int of(int x) const { return x < warps * first ? x / first : warps + (x - warps * first) / rest; }
+};
+
+template <int D, int kThreads>
+__device__ __forceinline__ void join_parts(const AttendLaunch& P, float (*s_ml)[2], float4 (*s_v)[D / 4], int u0, int sharers, int rows, int h,
+                                           int64_t out_row) {
+  constexpr int kWarps = kThreads / 32, kWords = D / 4;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t size = rows * (D + 4);
+  auto part = [&](int k) { return P.parts + (2 * static_cast<int64_t>(u0 + k) + (k == 0 ? 1 : 0)) * size; };
+  float m = -INFINITY, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = warp; k0 < sharers; k0 += kJoin * kWarps) {
+    float4 a[kJoin];  // all loads under way before the first is used
+    float2 ml[kJoin];
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+      ml[j] = make_float2(-INFINITY, 0.f);
+      a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + j * kWarps < sharers) {
+        const float* r = part(k0 + j * kWarps);
+        ml[j] = __ldcg(reinterpret_cast<const float2*>(r + rows * D) + h);
+        if (lane < kWords) a[j] = __ldcg(reinterpret_cast<const float4*>(r + h * D) + lane);
+      }
+    }
+    float n = m;
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) n = fmaxf(n, ml[j].x);
+    const float base = n == -INFINITY ? 0.f : n, fo = exp2_fast(m - base);
+    m = n;
+    l *= fo;
+    v = f4_scale(fo, v);
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+      const float f = exp2_fast(ml[j].x - base);
+      l = fmaf(f, ml[j].y, l);
+      v = f4_axpy(f, a[j], v);
+    }
+  }
+  if (lane < kWords) s_v[warp][lane] = v;
+  if (lane == 0) {
+    s_ml[warp][0] = m;
+    s_ml[warp][1] = l;
+  }
+  __syncthreads();
+  if (tid < kWords) {
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][0]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2_fast(s_ml[w][0] - base);
+      l = fmaf(f, s_ml[w][1], l);
+      v = f4_axpy(f, s_v[w][tid], v);
+    }
+    st4_rt(P.out, out_row * D + 4 * tid, f4_scale(1.f / l, v), P.dtype);
+  }
+  __syncthreads();  // the next pair's parts go there
+}
+
+// The same for up to kJoin parts: a thread reads all of them for its words of the pair's output.
+template <int D, int kThreads>
+__device__ __forceinline__ void join_few(const AttendLaunch& P, int u0, int sharers, int rows, int heads_here, int64_t out_row) {
+  const int64_t size = rows * (D + 4);
+  for (int t = threadIdx.x; t < heads_here * (D / 4); t += kThreads) {
+    const int h = t / (D / 4);
+    float4 a[kJoin];
+    float2 ml[kJoin];
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+      ml[j] = make_float2(-INFINITY, 0.f);
+      a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < sharers) {
+        const float* r = P.parts + (2 * static_cast<int64_t>(u0 + j) + (j == 0 ? 1 : 0)) * size;
+        ml[j] = __ldcg(reinterpret_cast<const float2*>(r + rows * D) + h);
+        a[j] = __ldcg(reinterpret_cast<const float4*>(r) + t);
+      }
+    }
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) m = fmaxf(m, ml[j].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j) {
+      const float f = exp2_fast(ml[j].x - base);
+      l = fmaf(f, ml[j].y, l);
+      v = f4_axpy(f, a[j], v);
+    }
+    st4_rt(P.out, out_row * D + 4 * t, f4_scale(1.f / l, v), P.dtype);
+  }
+}
+
+// Joins the parts of the pairs that lie in several units: a block for a pair of few parts, and one for each
+// head of a pair of many.  What depends on the lengths alone is done before the first kernel ends.
+template <int D, int kThreads>
+__global__ void __launch_bounds__(kThreads) cow_kv8_join_kernel(const __grid_constant__ AttendLaunch P) {
+  constexpr int kWarps = kThreads / 32, kWords = D / 4;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* s_prefix = reinterpret_cast<int*>(smem);
+  __shared__ int2 s_scan[kWarps];
+  __shared__ float s_ml[kWarps][2];
+  __shared__ float4 s_v[kWarps][kWords];
+  const int h = blockIdx.y, pairs = P.kv_heads * P.chunks, rows = min(P.group, kAttendHeads);
+  const int2 found = scan_pages<kThreads>(P, s_prefix, s_scan);
+  const Units units = Units::make(found.x * pairs, P.warps, P.slots);
+  bool waited = false;
+  if (found.y > kAlignedPages || P.requests * pairs * kAttendWarps > P.warps) {  // else each pair had its own block
+    for (int i = blockIdx.x; i < P.requests * pairs; i += gridDim.x) {
+      const int b = i / pairs, pair = i - b * pairs, np = s_prefix[b + 1] - s_prefix[b];
+      if (np == 0) continue;
+      const int pair0 = s_prefix[b] * pairs + pair * np;
+      const int u0 = units.of(pair0), sharers = units.of(pair0 + np - 1) - u0 + 1;
+      const int kv_head = P.chunks == 1 ? pair : pair / P.chunks, head0 = (pair - kv_head * P.chunks) * kAttendHeads;
+      const int heads_here = min(kAttendHeads, P.group - head0);
+      const int64_t row = static_cast<int64_t>(b) * P.heads + kv_head * P.group + head0;
+      if (sharers == 1 || h >= (sharers <= kJoin ? 1 : heads_here)) continue;
+      if (!waited) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
+        waited = true;
+      }
+      if (sharers <= kJoin) join_few<D, kThreads>(P, u0, sharers, rows, heads_here, row);
+      else join_parts<D, kThreads>(P, s_ml, s_v, u0, sharers, rows, h, row + h);
+    }
+  }
+  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // this kernel ends after the first
+}
+
+template <int D, bool kSplit>
+__global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend_kernel(const __grid_constant__ AttendLaunch P) {
+  using S = PageShape<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  uint8_t* s_keys = smem + warp * 2 * S::kBytes;
+  uint8_t* s_values = s_keys + S::kBytes;
+  int* s_prefix = reinterpret_cast<int*>(smem + kAttendWarps * 2 * S::kBytes);  // [requests + 1] pages before
+  __shared__ int2 s_scan[kAttendWarps];
+  __shared__ uint64_t s_bars[kAttendWarps][2];  // the warp's keys, values are there
+  const int R = P.requests, pairs = P.kv_heads * P.chunks, rows = min(P.group, kAttendHeads);
+
+  if (lane == 0) {
+    mbar_init(&s_bars[warp][0], 1);
+    mbar_init(&s_bars[warp][1], 1);
+  }
+  const int most = static_cast<int>(P.max_blocks) * kPage;
+  const int2 found = scan_pages<kAttendThreads>(P, s_prefix, s_scan);
+  const int all = found.x, longest = found.y;
 
   // a request without tokens: zeros
-  for (int b = blockIdx.x; b < R; b += G) {
+  for (int b = blockIdx.x; b < R; b += gridDim.x) {
     if (s_prefix[b + 1] == s_prefix[b])
       for (int i = tid; i < P.heads * D / 4; i += kAttendThreads)
         st4_rt(P.out, static_cast<int64_t>(b) * P.heads * D + 4 * i, make_float4(0.f, 0.f, 0.f, 0.f), P.dtype);
   }
 
-  // this block's run of the list (request, pair, page); at least a page for each warp
-  const int64_t total = static_cast<int64_t>(all) * pairs;
-  const int64_t share = max((total + G - 1) / G, static_cast<int64_t>(kAttendWarps));
-  int64_t here = blockIdx.x * share;
-  const int64_t end = min(here + share, total);
-
-  while (here < end) {
-    // which request, pair and page the run stands at
-    int lo = 0, hi = R;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (static_cast<int64_t>(s_prefix[mid]) * pairs <= here) lo = mid; else hi = mid;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // this warp's first unit of the list
+  const int total = all * pairs, warps = gridDim.x * kAttendWarps;
+  const bool aligned = longest <= kAlignedPages && R * pairs <= static_cast<int>(gridDim.x);
+  const Units units = Units::make(total, warps, P.slots);
+  int unit = blockIdx.x * kAttendWarps + warp, x0 = 0, x1 = 0;
+  if (aligned) {
+    const int b = blockIdx.x / pairs;
+    if (b < R) {
+      const int np = s_prefix[b + 1] - s_prefix[b];
+      x0 = s_prefix[b] * pairs + blockIdx.x % pairs * np;
+      x1 = x0 + np * (warp + 1) / kAttendWarps;
+      x0 += np * warp / kAttendWarps;
     }
-    const int b = lo, np = s_prefix[b + 1] - s_prefix[b];
-    const int64_t before = static_cast<int64_t>(s_prefix[b]) * pairs;
-    const int pair = static_cast<int>((here - before) / np);
-    const int64_t pair_begin = before + static_cast<int64_t>(pair) * np;
-    const int p_first = static_cast<int>(here - pair_begin);
-    const int p_last = static_cast<int>(min(static_cast<int64_t>(np), end - pair_begin));
-    here = pair_begin + p_last;
-    const int kv_head = pair / P.chunks, chunk = pair % P.chunks;
-    const int length = min(P.lengths[b], most);
-    const int head0 = kv_head * P.group + chunk * kAttendHeads;
-    const int heads_here = min(kAttendHeads, P.group - chunk * kAttendHeads);
-    const int32_t* table = P.tables + b * P.max_blocks;
+  } else {
+    x0 = units.begin(unit);
+    x1 = units.begin(unit + 1);
+  }
 
-    auto tile_of = [&](int p) {
-      int page = table[p];
-      if (page < 0 || page >= P.pages) {
-        if (lane == 0) atomicOr(P.status, COW_ST_ROW_RANGE);
-        page = 0;
-      }
-      return static_cast<int64_t>(page) * P.kv_heads + kv_head;
-    };
-
-    int p = p_first + warp;
-    int64_t tile = 0;
-    float ks = 0.f, vs = 0.f;
-    if (p < p_last) {
-      tile = tile_of(p);
-      copy_keys<D>(smem_addr(s_keys), P.key_codes + tile * S::kBytes, lane);
-      copies_commit();
-      copy_values<D>(smem_addr(s_values), P.value_codes + tile * S::kBytes, lane);
-      copies_commit();
-      ks = P.key_scales[tile];
-      vs = P.value_scales[tile];
+  // Lane i holds entry held_from + i of the block table of the pair that was last asked for.
+  int held = 0, held_from = 0;
+  auto tile_of = [&](const Place& w, bool new_pair) {
+    if (new_pair || w.p - held_from >= 32) {
+      held_from = w.p;
+      if (held_from + lane < w.np) held = P.tables[w.b * P.max_blocks + held_from + lane];
     }
+    int page = __shfl_sync(kFull, held, w.p - held_from);
+    if (page < 0 || page >= P.pages) {
+      if (lane == 0) atomicOr(P.status, COW_ST_ROW_RANGE);
+      page = 0;
+    }
+    return static_cast<int64_t>(page) * P.kv_heads + w.pair / P.chunks;
+  };
+  uint64_t* bars = s_bars[warp];
+  auto copy = [&](int which, int64_t tile) {  // what was in its place has been read by all lanes
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bars[which], S::kBytes);
+      bulk_row_copy(which ? s_values : s_keys, (which ? P.value_codes : P.key_codes) + tile * S::kBytes, S::kBytes, &bars[which]);
+    }
+  };
 
-    // the query of column g as operand columns, scaled so that its largest element is in [2^14, 2^15)
+  if (x0 < x1) {
+    Place now = place_of(s_prefix, R, pairs, x0);
+    const int64_t tile = tile_of(now, true);
+    copy(0, tile);
+    copy(1, tile);
+    unsigned parity = 0;
+    float ks = P.key_scales[tile], vs = P.value_scales[tile];
+    unsigned grabbed = 0;  // lane 0: the unit after this one
+    if (!aligned && lane == 0) grabbed = atomicAdd(P.taken, 1u);
+    bool began = now.p == 0;  // the pair's first page is in this unit
+
     unsigned qa[S::kKeySteps][2], qb[kSplit ? S::kKeySteps : 1][2];
-    float unscale;
-    {
-      float x[S::kKeySteps][4];
-      float big = 0.f;
-      const bool there = g < heads_here;
-      const int64_t row = b * P.q_request_stride + static_cast<int64_t>(head0 + (there ? g : 0)) * P.q_head_stride;
+    float f0 = 0.f, f1 = 0.f, m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
+    float o[D / 16][4];
+    int ve = 0, length = 0;  // the output is held in units of 2^ve
+    bool fresh = true;
+
+    for (int x = x0;;) {
+      if (fresh) {
+        // a new pair: the query of column g as operand columns, scaled so that its largest element is in [2^14, 2^15)
+        length = min(P.lengths[now.b], most);
+        const int head0 = now.pair / P.chunks * P.group + now.pair % P.chunks * kAttendHeads;
+        const bool there = g < min(kAttendHeads, P.group - now.pair % P.chunks * kAttendHeads);
+        const int64_t row = now.b * P.q_request_stride + static_cast<int64_t>(head0 + (there ? g : 0)) * P.q_head_stride;
+        float v[S::kKeySteps][4];
+        float big = 0.f;
 #pragma unroll
-      for (int k = 0; k < S::kKeySteps; ++k) {
-        const int h = k / 4;
-        const int d = h < S::kWhole ? 64 * h + 16 * c + 4 * (k % 4) : 64 * S::kWhole + 8 * c + 4 * (k % 2);
-        const float4 v = ld4_rt(P.q, row + d, P.dtype);
-        x[k][0] = there ? v.x : 0.f;
-        x[k][1] = there ? v.y : 0.f;
-        x[k][2] = there ? v.z : 0.f;
-        x[k][3] = there ? v.w : 0.f;
+        for (int k = 0; k < S::kKeySteps; ++k) {
+          const int h = k / 4;
+          const int d = h < S::kWhole ? 64 * h + 16 * c + 4 * (k % 4) : 64 * S::kWhole + 8 * c + 4 * (k % 2);
+          const float4 q = ld4_rt(P.q, row + d, P.dtype);
+          v[k][0] = there ? q.x : 0.f;
+          v[k][1] = there ? q.y : 0.f;
+          v[k][2] = there ? q.z : 0.f;
+          v[k][3] = there ? q.w : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (fabsf(x[k][i]) < INFINITY) big = fmaxf(big, fabsf(x[k][i]));
+          for (int i = 0; i < 4; ++i)
+            if (fabsf(v[k][i]) < INFINITY) big = fmaxf(big, fabsf(v[k][i]));
+        }
+        big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
+        const int e = min(max(14 - exponent_of(big), -100), 100);
+        const float up = pow2(e), unscale = pow2(-e) * P.scale_log2;
+#pragma unroll
+        for (int k = 0; k < S::kKeySteps; ++k) {
+          qa[k][0] = pack_half2(v[k][0] * up, v[k][1] * up);
+          qa[k][1] = pack_half2(v[k][2] * up, v[k][3] * up);
+          if constexpr (kSplit) {
+            qb[k][0] = pack_rest2(v[k][0] * up, v[k][1] * up, qa[k][0]);
+            qb[k][1] = pack_rest2(v[k][2] * up, v[k][3] * up, qa[k][1]);
+          }
+        }
+        // this lane's score columns are heads 2c and 2c + 1
+        f0 = __shfl_sync(kFull, unscale, 8 * c);
+        f1 = __shfl_sync(kFull, unscale, 8 * c + 4);
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        ve = exponent_of(vs);
+        fresh = false;
       }
-      big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
-      const int e = min(max(14 - exponent_of(big), -100), 100);
-      const float up = pow2(e);
-      unscale = pow2(-e);
-#pragma unroll
-      for (int k = 0; k < S::kKeySteps; ++k) {
-        qa[k][0] = pack_half2(x[k][0] * up, x[k][1] * up);
-        qa[k][1] = pack_half2(x[k][2] * up, x[k][3] * up);
-        if constexpr (kSplit) {
-          qb[k][0] = pack_rest2(x[k][0] * up, x[k][1] * up, qa[k][0]);
-          qb[k][1] = pack_rest2(x[k][2] * up, x[k][3] * up, qa[k][1]);
+
+      // the next page, maybe of the next pair or unit
+      const bool unit_ends = x + 1 == x1;
+      bool more = !unit_ends;
+      Place next = now;
+      int64_t next_tile = 0;
+      int next_unit = unit, next_x = x + 1;
+      if (!unit_ends) {
+        if (++next.p == next.np) {
+          next.p = 0;
+          if (++next.pair == pairs) {
+            next.pair = 0;
+            do ++next.b;
+            while (s_prefix[next.b + 1] == s_prefix[next.b]);  // there is another page, so another request
+            next.np = s_prefix[next.b + 1] - s_prefix[next.b];
+          }
+        }
+      } else if (!aligned) {
+        next_unit = warps + static_cast<int>(__shfl_sync(kFull, grabbed, 0));
+        next_x = units.begin(next_unit);
+        more = next_x < total;
+        if (more) next = place_of(s_prefix, R, pairs, next_x);
+      }
+      if (more) {
+        const bool new_pair = next.pair != now.pair || next.b != now.b || unit_ends;
+        next_tile = tile_of(next, new_pair);
+        if (new_pair) {  // its queries, on their way to where the next turn reads them
+          const int h = next.pair / P.chunks * P.group + next.pair % P.chunks * kAttendHeads + min(g, min(kAttendHeads, P.group - next.pair % P.chunks * kAttendHeads) - 1);
+          const char* q = P.q + (next.b * P.q_request_stride + h * P.q_head_stride) * (P.dtype == COW_F32 ? 4 : 2);
+          for (int d = 128 * c; d < D * (P.dtype == COW_F32 ? 4 : 2); d += 512) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + d));
         }
       }
-    }
-    // this lane's score columns are heads 2c and 2c + 1
-    const float f0 = __shfl_sync(kFull, unscale, 8 * c) * P.scale_log2;
-    const float f1 = __shfl_sync(kFull, unscale, 8 * c + 4) * P.scale_log2;
 
-    float o[D / 16][4];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    int ve = 0;  // the output is held in units of 2^ve
-
-    for (; p < p_last; p += kAttendWarps) {
-      const int next = p + kAttendWarps;
-      const bool more = next < p_last;
-      int64_t next_tile = 0;
-      if (more) next_tile = tile_of(next);
-
-      copies_wait<1>();  // the keys are here
+      // A wait that gives up is reported and the page taken as it is.
+      if (!mbar_wait(&bars[0], parity, kSpinLimit) && lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
       float s[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        const uint8_t* chunk0 = s_keys + lane * 16;
+        const int token = (g >> 1) * 16 + 4 * t + (g & 1);
 #pragma unroll
         for (int h = 0; h < S::kWhole; ++h) {
-          const uint4 a = *reinterpret_cast<const uint4*>(chunk0 + ((2 * t) * S::kWhole + h) * 512);
-          const uint4 z = *reinterpret_cast<const uint4*>(chunk0 + ((2 * t + 1) * S::kWhole + h) * 512);
+          const uint4 a = *reinterpret_cast<const uint4*>(s_keys + key_at<D>(token, 64 * h + 16 * c));
+          const uint4 z = *reinterpret_cast<const uint4*>(s_keys + key_at<D>(token + 2, 64 * h + 16 * c));
           const unsigned aw[4] = {a.x, a.y, a.z, a.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -608,9 +817,8 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
           }
         }
         if constexpr (S::kHalf) {
-          const uint8_t* chunk1 = s_keys + S::kWhole * 64 * kPage + lane * 8;
-          const uint2 a = *reinterpret_cast<const uint2*>(chunk1 + (2 * t) * 256);
-          const uint2 z = *reinterpret_cast<const uint2*>(chunk1 + (2 * t + 1) * 256);
+          const uint2 a = *reinterpret_cast<const uint2*>(s_keys + key_at<D>(token, 64 * S::kWhole + 8 * c));
+          const uint2 z = *reinterpret_cast<const uint2*>(s_keys + key_at<D>(token + 2, 64 * S::kWhole + 8 * c));
           const unsigned aw[2] = {a.x, a.y}, zw[2] = {z.x, z.y};
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -621,11 +829,10 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
           }
         }
       }
-      if (more) copy_keys<D>(smem_addr(s_keys), P.key_codes + next_tile * S::kBytes, lane);
-      copies_commit();
+      if (more) copy(0, next_tile);
 
       // scores, the page's maximum, probabilities
-      const int left = length - p * kPage;  // tokens of this page, if below 64
+      const int left = length - now.p * kPage;  // tokens of this page, if below 64
       const float fk0 = f0 * ks, fk1 = f1 * ks;
       float big0 = -INFINITY, big1 = -INFINITY;
 #pragma unroll
@@ -639,9 +846,9 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
         big1 = fmaxf(big1, fmaxf(s[t][1], s[t][3]));
       }
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) {
-        big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, x));
-        big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, x));
+      for (int y = 4; y < 32; y <<= 1) {
+        big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, y));
+        big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, y));
       }
       const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
       // where every score so far is -inf, exponents are taken from 0: probabilities 0, no NaN
@@ -653,7 +860,6 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
       l1 *= a1;
       // The output follows the page's value scale; a page 2^64 below the others keeps theirs and
       // its probabilities shrink instead, so no factor overflows.
-      if (p == p_first + warp) ve = exponent_of(vs);
       int step = ve - exponent_of(vs);
       float shrink = 1.f;
       if (step > 64) {
@@ -687,11 +893,12 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
         }
       }
 
-      copies_wait<1>();  // the values are here
+      if (!mbar_wait(&bars[1], parity, kSpinLimit) && lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+      parity ^= 1;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        uint4 a = *reinterpret_cast<const uint4*>(s_values + ((2 * i) * 32 + lane) * 16);
-        uint4 z = *reinterpret_cast<const uint4*>(s_values + ((2 * i + 1) * 32 + lane) * 16);
+        const uint4 a = *reinterpret_cast<const uint4*>(s_values + (16 * i + g) * kPage + 16 * c);
+        const uint4 z = *reinterpret_cast<const uint4*>(s_values + (16 * i + 8 + g) * kPage + 16 * c);
         unsigned aw[4] = {a.x, a.y, a.z, a.w}, zw[4] = {z.x, z.y, z.z, z.w};
         if (left < kPage) {  // codes past the last token may be anything, NaN among them: 0 * NaN is not 0
 #pragma unroll
@@ -710,102 +917,101 @@ __global__ void __launch_bounds__(kAttendThreads) cow_kv8_attend_kernel(const __
         }
       }
       if (more) {
-        copy_values<D>(smem_addr(s_values), P.value_codes + next_tile * S::kBytes, lane);
+        copy(1, next_tile);
         ks = P.key_scales[next_tile];
         vs = P.value_scales[next_tile];
       }
-      copies_commit();
-    }
-    copies_wait<0>();
-    // the sums over this warp's lanes
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      l0 += __shfl_xor_sync(kFull, l0, x);
-      l1 += __shfl_xor_sync(kFull, l1, x);
-    }
 
-    // ---- the block's four warps meet in shared memory (their pages are used up)
-    __syncwarp();
-    float* mine = reinterpret_cast<float*>(s_keys);  // [8][D + 2]
-    const float unit = pow2(min(max(ve, -126), 127));
+      const bool ended = now.p + 1 == now.np;
+      if (ended || unit_ends) {
+        // the pair, or this unit's part of it, is done
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      mine[(2 * c) * kRow + 16 * i + g] = o[i][0] * unit;
-      mine[(2 * c + 1) * kRow + 16 * i + g] = o[i][1] * unit;
-      mine[(2 * c) * kRow + 16 * i + g + 8] = o[i][2] * unit;
-      mine[(2 * c + 1) * kRow + 16 * i + g + 8] = o[i][3] * unit;
-    }
-    if (g == 0) {
-      mine[(2 * c) * kRow + D] = m0;
-      mine[(2 * c) * kRow + D + 1] = l0;
-      mine[(2 * c + 1) * kRow + D] = m1;
-      mine[(2 * c + 1) * kRow + D + 1] = l1;
-    }
-    __syncthreads();
-    const bool whole = p_first == 0 && p_last == np;
-    const int64_t pair_end = pair_begin + np;
-    const int64_t first_block = pair_begin / share;
-    const int sharers = static_cast<int>((pair_end - 1) / share - first_block) + 1;
-    float* partial = P.partials + (2 * static_cast<int64_t>(blockIdx.x) + (p_first == 0 ? 1 : 0)) * (kAttendHeads * kRow);
-    for (int i = tid; i < heads_here * D; i += kAttendThreads) {
-      const int h = i / D, d = i % D;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, reinterpret_cast<float*>(smem + w * 2 * S::kBytes)[h * kRow + D]);
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f, v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kAttendWarps; ++w) {
-        const float* r = reinterpret_cast<float*>(smem + w * 2 * S::kBytes) + h * kRow;
-        const float f = exp2_fast(r[D] - base);
-        l = fmaf(f, r[D + 1], l);
-        v = fmaf(f, r[d], v);
-      }
-      if (whole) {
-        const float y = v / l;
-        const int64_t at_out = (static_cast<int64_t>(b) * P.heads + head0 + h) * D + d;
-        if (P.dtype == COW_F32) reinterpret_cast<float*>(P.out)[at_out] = y;
-        else if (P.dtype == COW_BF16) reinterpret_cast<__nv_bfloat16*>(P.out)[at_out] = __float2bfloat16_rn(y);
-        else reinterpret_cast<__half*>(P.out)[at_out] = __float2half_rn(y);
-      } else {
-        partial[h * kRow + d] = v;
-        if (d == 0) {
-          partial[h * kRow + D] = m;
-          partial[h * kRow + D + 1] = l;
+        for (int y = 4; y < 32; y <<= 1) {
+          l0 += __shfl_xor_sync(kFull, l0, y);
+          l1 += __shfl_xor_sync(kFull, l1, y);
         }
-      }
-    }
-    if (!whole) {
-      // the block that arrives last joins the pair's parts, in the order of its pages
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        unsigned* word = P.arrived + static_cast<int64_t>(b) * pairs + pair;
-        s_last = atomicInc(word, static_cast<unsigned>(sharers - 1)) == static_cast<unsigned>(sharers - 1);
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        for (int i = tid; i < heads_here * D; i += kAttendThreads) {
-          const int h = i / D, d = i % D;
-          float m = -INFINITY, l = 0.f, v = 0.f;
-          for (int k = 0; k < sharers; ++k) {
-            const float* r = P.partials + (2 * (first_block + k) + (k == 0 ? 1 : 0)) * (kAttendHeads * kRow) + h * kRow;
-            const float rm = __ldcg(r + D), n = fmaxf(m, rm), base = n == -INFINITY ? 0.f : n;
-            const float fo = exp2_fast(m - base), fr = exp2_fast(rm - base);
-            l = l * fo + __ldcg(r + D + 1) * fr;
-            v = v * fo + __ldcg(r + d) * fr;
-            m = n;
+        const float scale = pow2(min(max(ve, -126), 127));
+        const int chunk = now.pair % P.chunks, heads_here = min(kAttendHeads, P.group - chunk * kAttendHeads);
+        const int64_t row = static_cast<int64_t>(now.b) * P.heads + now.pair / P.chunks * P.group + chunk * kAttendHeads;
+        if (began && ended && !aligned) {
+          const float y0 = scale / l0, y1 = scale / l1;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            if (2 * c < heads_here) {
+              store_out(P, (row + 2 * c) * D + 16 * i + g, o[i][0] * y0);
+              store_out(P, (row + 2 * c) * D + 16 * i + g + 8, o[i][2] * y0);
+            }
+            if (2 * c + 1 < heads_here) {
+              store_out(P, (row + 2 * c + 1) * D + 16 * i + g, o[i][1] * y1);
+              store_out(P, (row + 2 * c + 1) * D + 16 * i + g + 8, o[i][3] * y1);
+            }
           }
-          const float y = v / l;
-          const int64_t at_out = (static_cast<int64_t>(b) * P.heads + head0 + h) * D + d;
-          if (P.dtype == COW_F32) reinterpret_cast<float*>(P.out)[at_out] = y;
-          else if (P.dtype == COW_BF16) reinterpret_cast<__nv_bfloat16*>(P.out)[at_out] = __float2bfloat16_rn(y);
-          else reinterpret_cast<__half*>(P.out)[at_out] = __float2half_rn(y);
+        } else {
+          if (aligned) __syncwarp();  // this warp's pages are used up
+          float* mine = aligned ? reinterpret_cast<float*>(s_keys) : P.parts + static_cast<int64_t>(2 * unit + (began ? 1 : 0)) * (rows * (D + 4));
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            if (2 * c < rows) {
+              mine[(2 * c) * D + 16 * i + g] = o[i][0] * scale;
+              mine[(2 * c) * D + 16 * i + g + 8] = o[i][2] * scale;
+            }
+            if (2 * c + 1 < rows) {
+              mine[(2 * c + 1) * D + 16 * i + g] = o[i][1] * scale;
+              mine[(2 * c + 1) * D + 16 * i + g + 8] = o[i][3] * scale;
+            }
+          }
+          if (g == 0) {
+            float2* ml = reinterpret_cast<float2*>(mine + rows * D);
+            if (2 * c < rows) ml[2 * c] = make_float2(m0, l0);
+            if (2 * c + 1 < rows) ml[2 * c + 1] = make_float2(m1, l1);
+          }
         }
+        began = true;
+        fresh = true;
       }
+      if (!more) break;
+      if (unit_ends) {
+        unit = next_unit;
+        x1 = units.begin(unit + 1);
+        began = next.p == 0;
+        if (lane == 0) grabbed = atomicAdd(P.taken, 1u);
+      }
+      x = next_x;
+      now = next;
     }
-    __syncthreads();  // shared memory is free for the next run
+  }
+
+  if (!aligned) {
+    // the last warp to end leaves the count of units as it was
+    if (lane == 0) {
+      __threadfence();
+      if (atomicInc(P.taken + 1, static_cast<unsigned>(warps - 1)) == static_cast<unsigned>(warps - 1)) *P.taken = 0;
+    }
+    return;
+  }
+  // ---- the warps' parts of the block's pair
+  const int b = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  if (b >= R || s_prefix[b + 1] == s_prefix[b]) return;  // the whole block
+  __syncthreads();
+  const int np = s_prefix[b + 1] - s_prefix[b];
+  const int chunk = pair % P.chunks, heads_here = min(kAttendHeads, P.group - chunk * kAttendHeads);
+  const int64_t row = static_cast<int64_t>(b) * P.heads + pair / P.chunks * P.group + chunk * kAttendHeads;
+  for (int t = tid; t < heads_here * (D / 4); t += kAttendThreads) {
+    const int h = t / (D / 4);
+    float m = -INFINITY, l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kAttendWarps; ++w) {
+      if (np * w / kAttendWarps == np * (w + 1) / kAttendWarps) continue;  // no page
+      const float* part = reinterpret_cast<const float*>(smem + w * 2 * S::kBytes);
+      const float2 ml = reinterpret_cast<const float2*>(part + rows * D)[h];
+      const float n = fmaxf(m, ml.x), base = n == -INFINITY ? 0.f : n;
+      const float fo = exp2_fast(m - base), fr = exp2_fast(ml.x - base);
+      l = l * fo + ml.y * fr;
+      v = f4_axpy(fr, reinterpret_cast<const float4*>(part)[t], f4_scale(fo, v));
+      m = n;
+    }
+    st4_rt(P.out, row * D + 4 * t, f4_scale(1.f / l, v), P.dtype);
   }
 }
 
@@ -836,11 +1042,21 @@ AttendFn attend_fn(int width, bool split) {
   return split ? cow_kv8_attend_kernel<128, true> : cow_kv8_attend_kernel<128, false>;
 }
 
-constexpr int kMaxAttendBlocks = 148 * 16;  // partials are sized for this many, more never run
+template <int kThreads>
+AttendFn join_fn(int width) {
+  if (width == 32) return cow_kv8_join_kernel<32, kThreads>;
+  if (width == 64) return cow_kv8_join_kernel<64, kThreads>;
+  return width == 96 ? cow_kv8_join_kernel<96, kThreads> : cow_kv8_join_kernel<128, kThreads>;
+}
 
-// bytes of the partials, then the arrival words
-int64_t partial_bytes(int width) {
-  return static_cast<int64_t>(2 * kMaxAttendBlocks) * kAttendHeads * (width + 2) * sizeof(float);
+// Blocks of a launch at most: what 168 (128) registers a thread let an SM hold.
+int max_attend_blocks(int width) { return 148 * (width > 64 ? 3 : 4); }
+// Units of W warps: W of floor(3/4 of a warp's share), at least 1, and what is left in eighths of a share
+// rounded up, at least 2.  Left are at most total / 4 + W pages: with total <= 16 W 2.5 W units of 2, above it
+// (total / 4 + W) / (total / 8 W) <= 2.5 W, and one that is not full.
+int64_t max_units(int width) { return int64_t{4} * max_attend_blocks(width) * kAttendWarps; }
+int64_t parts_bytes(int width, int group) {
+  return 2 * max_units(width) * (group < kAttendHeads ? group : kAttendHeads) * (width + 4) * static_cast<int64_t>(sizeof(float));
 }
 
 }  // namespace
@@ -895,8 +1111,7 @@ int cow_kv8_read(const cow_kv_pages* cache, int32_t layer, const int32_t* slots,
 
 int64_t cow_kv8_attend_workspace_bytes(const cow_kv_pages* cache, int32_t heads) {
   if (!cache || !shape_ok(cache) || heads < 1 || heads % cache->kv_heads) return -1;
-  const int64_t chunks = (heads / cache->kv_heads + kAttendHeads - 1) / kAttendHeads;
-  return partial_bytes(cache->width) + cache->requests * cache->kv_heads * chunks * static_cast<int64_t>(sizeof(unsigned));
+  return 16 + parts_bytes(cache->width, heads / cache->kv_heads);
 }
 
 int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries, int64_t query_request_stride,
@@ -909,28 +1124,48 @@ int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries
   if (cache->requests == 0) return COW_OK;
   if (!rows_ok(queries, query_request_stride, query_head_stride, dtype) || !out || !aligned16(out) || !cache->lengths ||
       (cache->max_blocks > 0 && cache->pages > 0 &&
-       (!cache->block_tables || !cache->key_codes || !cache->value_codes || !cache->key_scales || !cache->value_scales)))
+       (!cache->block_tables || !cache->key_codes || !cache->value_codes || !aligned16(cache->key_codes) ||
+        !aligned16(cache->value_codes) || !cache->key_scales || !cache->value_scales)))
     return COW_ERR_INVALID;
   const int64_t max_blocks = cache->pages > 0 ? cache->max_blocks : 0;  // without pages nothing is cached
   const int64_t tiles = layer * cache->pages * cache->kv_heads, bytes = tiles * kPage * cache->width;
   const int group = heads / cache->kv_heads, chunks = (group + kAttendHeads - 1) / kAttendHeads;
-  AttendLaunch P{cache->key_codes + bytes, cache->value_codes + bytes, cache->key_scales + tiles,
-                 cache->value_scales + tiles, cache->block_tables, cache->lengths, static_cast<const char*>(queries),
-                 static_cast<char*>(out), static_cast<float*>(workspace),
-                 reinterpret_cast<unsigned*>(static_cast<char*>(workspace) + partial_bytes(cache->width)), cache->status,
-                 query_request_stride, query_head_stride, max_blocks, static_cast<int32_t>(cache->requests),
-                 cache->kv_heads, heads, group, chunks, static_cast<int32_t>(cache->pages), dtype,
-                 scale * 1.4426950408889634f};
   const AttendFn fn = attend_fn(cache->width, dtype == COW_F32);
-  // the prefix is sized for whole 1,024s of requests, so that few sizes are ever asked for
+  // the prefix is sized for whole 512s of requests, so that few sizes are ever asked for
   const size_t smem = static_cast<size_t>(kAttendWarps) * 2 * kPage * cache->width +
-                      sizeof(int) * ((static_cast<size_t>(cache->requests) / 1024 + 1) * 1024);
+                      sizeof(int) * ((static_cast<size_t>(cache->requests) / 512 + 1) * 512);
   const int resident = resident_blocks(reinterpret_cast<const void*>(fn), kAttendThreads, smem);
   if (!resident) return COW_ERR_CUDA;
   const int64_t most = cache->requests * max_blocks * cache->kv_heads * chunks;
-  const int64_t blocks = most < resident ? (most < 1 ? 1 : most) : resident;
-  fn<<<static_cast<unsigned>(blocks < kMaxAttendBlocks ? blocks : kMaxAttendBlocks), kAttendThreads, smem,
-       as_stream(stream)>>>(P);
+  if (most >= (int64_t{1} << 31) - (1 << 20) || cache->requests * cache->kv_heads * chunks >= (1 << 28)) return COW_ERR_UNSUPPORTED;
+  int64_t blocks = most < 1 ? 1 : most;
+  if (blocks > resident) blocks = resident;
+  if (blocks > max_attend_blocks(cache->width)) blocks = max_attend_blocks(cache->width);
+  const AttendLaunch P{cache->key_codes + bytes, cache->value_codes + bytes, cache->key_scales + tiles,
+                       cache->value_scales + tiles, cache->block_tables, cache->lengths, static_cast<const char*>(queries),
+                       static_cast<char*>(out), reinterpret_cast<float*>(static_cast<char*>(workspace) + 16),
+                       static_cast<unsigned*>(workspace), cache->status, query_request_stride, query_head_stride, max_blocks,
+                       2 * max_units(cache->width), static_cast<int32_t>(blocks * kAttendWarps),
+                       static_cast<int32_t>(cache->requests), cache->kv_heads, heads, group, chunks,
+                       static_cast<int32_t>(cache->pages), dtype, scale * 1.4426950408889634f};
+  fn<<<static_cast<unsigned>(blocks), kAttendThreads, smem, as_stream(stream)>>>(P);
+  if (launch_status() != COW_OK) return COW_ERR_CUDA;
+  // tables so short that every pair has a block of its own: nothing to join
+  if (max_blocks <= kAlignedPages && cache->requests * cache->kv_heads * chunks <= blocks) return COW_OK;
+  cudaLaunchConfig_t cfg = {};
+  const int rows = group < kAttendHeads ? group : kAttendHeads;
+  const int64_t all_pairs = cache->requests * cache->kv_heads * chunks, wide = kJoinColumns;
+  cfg.gridDim = dim3(static_cast<unsigned>(all_pairs < wide ? all_pairs : wide), static_cast<unsigned>(rows));
+  cfg.dynamicSmemBytes = sizeof(int) * (static_cast<size_t>(cache->requests) + 1);
+  const bool few = all_pairs <= kJoinFewPairs;
+  cfg.blockDim = dim3(few ? kJoinThreadsFew : kJoinThreadsMany);
+  cfg.stream = as_stream(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, few ? join_fn<kJoinThreadsFew>(cache->width) : join_fn<kJoinThreadsMany>(cache->width), P);
   return launch_status();
 }
 

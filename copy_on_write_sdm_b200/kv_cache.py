@@ -152,7 +152,8 @@ class PagedKVCache:
     """K/V of a batch of requests for ``layers`` attention layers, in pages of 64 tokens.
 
     Keys and values are e4m3 codes with one power-of-two scale per (layer, page, head): a
-    value is ``code * scale``.  ``value_pages`` hold a page's tokens side by side.  A page
+    value is ``code * scale``.  ``value_pages`` hold a page's tokens side by side, and ``key_pages`` of
+    width 128 the rows of odd tokens with their halves exchanged (``read`` undoes both).  A page
     id stands for one page in every layer, so one ``resize`` serves them all.
     ``free_pages`` is a stack with its top at ``free_count - 1``.  ``status_word`` collects
     device errors as the SDM pools' ``overflow_flag`` does; ``validate_invariants`` raises.

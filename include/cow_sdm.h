@@ -546,7 +546,8 @@ int cow_attention_mlp_decode(const float* tokens, const int64_t* positions, cons
  * cache in the activation type (copy_on_write_sdm/inference.py:293-306).
  * Pages of COW_PAGE_TOKENS tokens come from one stack that all layers share
  * (a page id stands for one page of every layer):
- *   key_codes    [layers, pages, kv_heads, 64, width]  e4m3
+ *   key_codes    [layers, pages, kv_heads, 64, width]  e4m3; of width 128, odd tokens' rows
+ *                with their two halves exchanged
  *   value_codes  [layers, pages, kv_heads, width, 64]  e4m3, a page's tokens side by side
  *   key_scales, value_scales [layers, pages, kv_heads] float32, powers of two
  *   block_tables [requests, max_blocks] int32          page of each block, -1 none
@@ -554,8 +555,10 @@ int cow_attention_mlp_decode(const float* tokens, const int64_t* positions, cons
  *   free_pages   [pages] int32                         free stack, top at free_pages[free_count-1]
  *   free_count, status, ticket   int32 device scalars (ticket: zero, left zero)
  * A value is code * scale of its page and head.  width is 32, 64, 96 or 128;
- * requests <= 8192, requests * max_blocks < 2^25, pages < 2^25.  Calls on one
- * cache that could overlap on the GPU are the caller's to order. */
+ * requests <= 8192, requests * max_blocks < 2^25, pages < 2^25, and for
+ * cow_kv8_attend requests * max_blocks * kv_heads * ceil(group / 8) below
+ * 2^31 - 2^20.  Calls on one cache that could overlap on the GPU are the
+ * caller's to order. */
 #define COW_PAGE_TOKENS 64
 #define COW_MAX_REQUESTS 8192
 
