@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int kPage = COW_PAGE_TOKENS;
-constexpr int kStoreThreads = 128;
+constexpr int kStoreThreads = 256;
 constexpr int kStoreWarps = kStoreThreads / 32;
 constexpr int kLeastExponent = -64;
 
@@ -57,44 +57,31 @@ __device__ __forceinline__ int key_at(int t, int d) {
   return t * D + (D == 128 ? d ^ ((t & 1) << 6) : d);
 }
 
-// 16 bytes of a tensor as floats
+// 16 bytes of a tensor: four 32-bit words of one or two elements
 template <int DT>
-struct Vec16;
-template <>
-struct Vec16<COW_F32> {
-  static constexpr int kElems = 4;
-  static __device__ __forceinline__ void get(uint4 u, float* x) {
-    x[0] = __uint_as_float(u.x);
-    x[1] = __uint_as_float(u.y);
-    x[2] = __uint_as_float(u.z);
-    x[3] = __uint_as_float(u.w);
-  }
-};
-template <>
-struct Vec16<COW_BF16> {
-  static constexpr int kElems = 8;
-  static __device__ __forceinline__ void get(uint4 u, float* x) {
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+struct Vec16 {
+  static constexpr int kElems = DT == COW_F32 ? 4 : 8;
+  static constexpr int kPerWord = kElems / 4;
+  static __device__ __forceinline__ void word(unsigned w, float* x) {
+    if constexpr (DT == COW_F32) {
+      x[0] = __uint_as_float(w);
+    } else if constexpr (DT == COW_BF16) {
+      x[0] = __uint_as_float(w << 16);
+      x[1] = __uint_as_float(w & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      x[0] = f.x;
+      x[1] = f.y;
     }
   }
-};
-template <>
-struct Vec16<COW_F16> {
-  static constexpr int kElems = 8;
   static __device__ __forceinline__ void get(uint4 u, float* x) {
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
+    word(u.x, x);
+    word(u.y, x + kPerWord);
+    word(u.z, x + 2 * kPerWord);
+    word(u.w, x + 3 * kPerWord);
   }
 };
+__device__ __forceinline__ unsigned word_of(uint4 u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
 template <int DT>
 __device__ __forceinline__ float most_of(uint4 u, float most) {
@@ -112,12 +99,15 @@ __device__ __forceinline__ float most_of(uint4 u, float most) {
 // store
 // --------------------------------------------------------------------------
 //
-// One block per (page piece, head) of the plan: the piece's tokens of keys, then of values,
+// One block per (page piece, head) of the plan and keys or values: the piece's tokens
 // are read once into registers, their largest magnitude gives the scale, and the codes are
 // written.  Keys: a thread's 16 bytes are neighbours of the next thread's.  Values: a lane
 // reads one 16-byte word of each of four neighbouring tokens and so holds whole 32-bit words
 // of four codes of the transposed page; two lanes share a 32-byte sector.
-// Bound: memory, (element size + 1) bytes for each element of keys and values.
+// Bound: memory, (element size + 1) bytes for each element of keys and values.  A block's time is mostly
+// latency (load, maximum, store), so many must be resident: 66,000 tokens of 8 heads of 128 in bf16 take 81 us with
+// 256 threads and five blocks an SM (5.0 TB/s), 100 us with 128 threads and six, 136 us with keys and
+// values in one block of 168 registers.
 
 struct StoreLaunch {
   uint8_t* codes[2];  // keys, values: this layer's pages
@@ -128,126 +118,118 @@ struct StoreLaunch {
   int32_t kv_heads, pages;
 };
 
-__device__ __forceinline__ float block_most(float most, float* s_red, int lane, int warp) {
+__device__ __forceinline__ float block_most(float most, float* s_most, int lane, int warp) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-  __syncthreads();  // the previous use of s_red is over
-  if (lane == 0) s_red[warp] = most;
+  if (lane == 0) s_most[warp] = most;
   __syncthreads();
-  most = s_red[0];
+  most = s_most[0];
 #pragma unroll
-  for (int w = 1; w < kStoreWarps; ++w) most = fmaxf(most, s_red[w]);
+  for (int w = 1; w < kStoreWarps; ++w) most = fmaxf(most, s_most[w]);
   return most;
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(kStoreThreads) cow_kv8_store_kernel(const __grid_constant__ StoreLaunch P) {
+__global__ void __launch_bounds__(kStoreThreads, DT == COW_F32 ? 3 : 5) cow_kv8_store_kernel(const __grid_constant__ StoreLaunch P) {
   constexpr int E = Vec16<DT>::kElems;
   constexpr int kVecs = D / E;                                          // 16-byte words per token
   constexpr int kKeyVecs = (kPage * kVecs + kStoreThreads - 1) / kStoreThreads;
   constexpr int kGroups = D / (2 * E);                                  // pairs of words per token
   constexpr int kValueGroups = (kGroups + kStoreWarps - 1) / kStoreWarps;
-  __shared__ float s_red[kStoreWarps];
+  __shared__ float s_most[kStoreWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int head = blockIdx.y;
+  const int head = blockIdx.y, which = blockIdx.z;
   if (static_cast<int>(blockIdx.x) >= P.plan[0]) return;
   const int4 piece = reinterpret_cast<const int4*>(P.plan + 4)[blockIdx.x];
   const int first = piece.x, tokens = piece.y, page = piece.z, offset = piece.w;
   if (page < 0 || page >= P.pages) return;
-  const int64_t tile = static_cast<int64_t>(page) * P.kv_heads + head;
+  const int64_t tile = static_cast<int64_t>(page) * P.kv_heads + head, stride = P.token_stride[which];
+  const char* src = P.x[which] + first * stride + head * P.head_stride[which];
+  uint8_t* dst = P.codes[which] + tile * (kPage * D);
+  float* scale = P.scales[which] + tile;
+  // the scale of a page that holds tokens already
+  const int old = offset > 0 ? exponent_of(*scale) : kLeastExponent;
 
-  // ---- keys
-  {
-    const char* src = P.x[0] + first * P.token_stride[0] + head * P.head_stride[0];
-    uint8_t* dst = P.codes[0] + tile * (kPage * D);
-    uint4 w[kKeyVecs];
-    float most = 0.f;
+  if (which == 0) {
+    uint4 k[kKeyVecs];
 #pragma unroll
     for (int i = 0; i < kKeyVecs; ++i) {
-      const int v = tid + i * kStoreThreads;
-      if (v < tokens * kVecs)
-        w[i] = __ldg(reinterpret_cast<const uint4*>(src + (v / kVecs) * P.token_stride[0]) + v % kVecs);
+      const int n = tid + i * kStoreThreads;
+      k[i] = make_uint4(0, 0, 0, 0);
+      if (n < tokens * kVecs) k[i] = __ldg(reinterpret_cast<const uint4*>(src + (n / kVecs) * stride) + n % kVecs);
     }
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kKeyVecs; ++i)
-      if (tid + i * kStoreThreads < tokens * kVecs) most = most_of<DT>(w[i], most);
-    int e = scale_exponent(block_most(most, s_red, lane, warp));
-    if (offset > 0) {
-      const int old = exponent_of(P.scales[0][tile]);
-      e = max(e, old);
-      if (e > old) {
-        const float ratio = e - old > 126 ? 0.f : pow2(old - e);
-        for (int i = tid; i < offset * D / 4; i += kStoreThreads) {
-          unsigned* word = reinterpret_cast<unsigned*>(dst) + i;
-          *word = recode4(*word, ratio);
-        }
+    for (int i = 0; i < kKeyVecs; ++i) most = most_of<DT>(k[i], most);
+    const int e = max(scale_exponent(block_most(most, s_most, lane, warp)), old);
+    if (offset > 0 && e > old) {  // codes that were there move to a larger scale
+      const float ratio = e - old > 126 ? 0.f : pow2(old - e);
+      for (int i = tid; i < offset * D / 4; i += kStoreThreads) {
+        unsigned* word = reinterpret_cast<unsigned*>(dst) + i;
+        *word = recode4(*word, ratio);
       }
     }
     const float inv = pow2(-e);
 #pragma unroll
     for (int i = 0; i < kKeyVecs; ++i) {
-      const int v = tid + i * kStoreThreads;
-      if (v < tokens * kVecs) {
+      const int n = tid + i * kStoreThreads;
+      if (n < tokens * kVecs) {
         float x[E];
-        Vec16<DT>::get(w[i], x);
-        unsigned* out = reinterpret_cast<unsigned*>(dst + key_at<D>(offset + v / kVecs, v % kVecs * E));
+        Vec16<DT>::get(k[i], x);
+        unsigned codes[E / 4];
 #pragma unroll
-        for (int j = 0; j < E; j += 4) out[j / 4] = encode4(x[j] * inv, x[j + 1] * inv, x[j + 2] * inv, x[j + 3] * inv);
+        for (int j = 0; j < E; j += 4) codes[j / 4] = encode4(x[j] * inv, x[j + 1] * inv, x[j + 2] * inv, x[j + 3] * inv);
+        uint8_t* out = dst + key_at<D>(offset + n / kVecs, n % kVecs * E);
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(out) = make_uint2(codes[0], codes[1]);
+        else *reinterpret_cast<unsigned*>(out) = codes[0];
       }
     }
-    __syncthreads();  // every thread has read the old scale
-    if (tid == 0) P.scales[0][tile] = pow2(e);
+    if (tid == 0) *scale = pow2(e);  // past the barrier in block_most: every thread has read the old one
+    return;
   }
 
-  // ---- values
-  {
-    const char* src = P.x[1] + head * P.head_stride[1];
-    uint8_t* dst = P.codes[1] + tile * (kPage * D);
-    const int t0 = (lane >> 1) * 4;  // this lane's four tokens of the page
-    uint4 w[kValueGroups][4];
-    float most = 0.f;
+  const int t0 = (lane >> 1) * 4;  // this lane's four tokens of the page
+  uint4 v[kValueGroups][4];
 #pragma unroll
-    for (int i = 0; i < kValueGroups; ++i) {
-      const int g = warp + i * kStoreWarps;
+  for (int i = 0; i < kValueGroups; ++i) {
+    const int g = warp + i * kStoreWarps;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = t0 + j - offset;
-        w[i][j] = make_uint4(0, 0, 0, 0);
-        if (g < kGroups && t >= 0 && t < tokens)
-          w[i][j] = __ldg(reinterpret_cast<const uint4*>(src + (first + t) * P.token_stride[1]) + 2 * g + (lane & 1));
-      }
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0 + j - offset;
+      v[i][j] = make_uint4(0, 0, 0, 0);
+      if (g < kGroups && t >= 0 && t < tokens) v[i][j] = __ldg(reinterpret_cast<const uint4*>(src + t * stride) + 2 * g + (lane & 1));
     }
+  }
+  float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kValueGroups; ++i)
+  for (int i = 0; i < kValueGroups; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) most = most_of<DT>(w[i][j], most);
-    int e = scale_exponent(block_most(most, s_red, lane, warp));
-    if (offset > 0) {
-      const int old = exponent_of(P.scales[1][tile]);
-      e = max(e, old);
-      if (e > old) {
-        const float ratio = e - old > 126 ? 0.f : pow2(old - e);
-        const int words = (offset + 3) / 4;  // the last may hold bytes past the old tokens: written after the barrier
-        for (int i = tid; i < D * words; i += kStoreThreads) {
-          unsigned* word = reinterpret_cast<unsigned*>(dst + (i / words) * kPage) + i % words;
-          *word = recode4(*word, ratio);
-        }
-      }
+    for (int j = 0; j < 4; ++j) most = most_of<DT>(v[i][j], most);
+  const int e = max(scale_exponent(block_most(most, s_most, lane, warp)), old);
+  if (offset > 0 && e > old) {
+    const float ratio = e - old > 126 ? 0.f : pow2(old - e);
+    const int words = (offset + 3) / 4;  // the last may hold bytes of new tokens: those are written after the barrier
+    for (int i = tid; i < D * words; i += kStoreThreads) {
+      unsigned* word = reinterpret_cast<unsigned*>(dst + (i / words) * kPage) + i % words;
+      *word = recode4(*word, ratio);
     }
     __syncthreads();
-    const float inv = pow2(-e);
+  }
+  const float inv = pow2(-e);
+  const int have = min(t0 + 4, offset + tokens) - max(t0, offset);
 #pragma unroll
-    for (int i = 0; i < kValueGroups; ++i) {
-      const int g = warp + i * kStoreWarps;
-      const int have = min(t0 + 4, offset + tokens) - max(t0, offset);
-      if (g < kGroups && have > 0) {
-        float x[4][E];
+  for (int i = 0; i < kValueGroups; ++i) {
+    const int g = warp + i * kStoreWarps;
+    if (g < kGroups && have > 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) Vec16<DT>::get(w[i][j], x[j]);
+      for (int w = 0; w < 4; ++w) {
+        float x[4][Vec16<DT>::kPerWord];
 #pragma unroll
-        for (int d = 0; d < E; ++d) {
+        for (int j = 0; j < 4; ++j) Vec16<DT>::word(word_of(v[i][j], w), x[j]);
+#pragma unroll
+        for (int d = 0; d < Vec16<DT>::kPerWord; ++d) {
           const unsigned codes = encode4(x[0][d] * inv, x[1][d] * inv, x[2][d] * inv, x[3][d] * inv);
-          uint8_t* out = dst + ((2 * g + (lane & 1)) * E + d) * kPage + t0;
+          uint8_t* out = dst + ((2 * g + (lane & 1)) * E + w * Vec16<DT>::kPerWord + d) * kPage + t0;
           if (have == 4) {
             *reinterpret_cast<unsigned*>(out) = codes;
           } else {
@@ -258,17 +240,19 @@ __global__ void __launch_bounds__(kStoreThreads) cow_kv8_store_kernel(const __gr
         }
       }
     }
-    if (tid == 0) P.scales[1][tile] = pow2(e);
   }
+  if (tid == 0) *scale = pow2(e);
 }
 
 // --------------------------------------------------------------------------
 // read
 // --------------------------------------------------------------------------
 //
-// One block per (32 slots, head).  Keys: a warp takes a slot, each lane four codes of its row.
-// Values: a lane takes a slot and the block walks the width, so neighbouring slots of a page
-// share each 32-byte sector; the codes cross shared memory to leave as rows.
+// One block per (32 list entries, head).  Keys: neighbouring threads take 16-byte words of a row, a row after
+// another.  Values: the entries' slots fall into columns, aligned groups of four tokens of a page; a thread
+// reads a column's word at four neighbouring widths, turns the 4 x 4 codes about, and they leave
+// through shared memory as rows.
+// Bound: memory, (1 + element size) bytes for each element.
 
 struct ReadLaunch {
   const uint8_t* codes[2];
@@ -276,46 +260,103 @@ struct ReadLaunch {
   char* out[2];
   const int32_t* slots;
   int64_t count;
-  int32_t kv_heads, pages, width, dtype;
+  int32_t kv_heads, pages;
 };
 
 constexpr int kReadSlots = 32;
+constexpr int kReadThreads = 128;
+static_assert(kReadSlots == 32, "the entries are one warp's");
 
-__global__ void __launch_bounds__(kStoreThreads) cow_kv8_read_kernel(const __grid_constant__ ReadLaunch P) {
-  __shared__ uint8_t s_codes[kReadSlots][128 + 4];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = P.width, head = blockIdx.y;
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kReadSlots;
-  const int here = static_cast<int>(min(static_cast<int64_t>(kReadSlots), P.count - base));
-  const int limit = P.pages * kPage;
-  // values: into shared memory, transposed
-  {
-    const int slot = lane < here ? P.slots[base + lane] : -1;
-    const bool ok = slot >= 0 && slot < limit;
-    const uint8_t* src = P.codes[1] + (static_cast<int64_t>(ok ? slot / kPage : 0) * P.kv_heads + head) * (kPage * D) +
-                         (ok ? slot % kPage : 0);
-    for (int d = warp; d < D; d += kStoreWarps) s_codes[lane][d] = ok ? src[d * kPage] : 0;
-  }
-  __syncthreads();
-  for (int i = warp; i < here; i += kStoreWarps) {
-    const int slot = P.slots[base + i];
-    const bool ok = slot >= 0 && slot < limit;
-    const int64_t tile = static_cast<int64_t>(ok ? slot / kPage : 0) * P.kv_heads + head;
-    const int64_t row = (base + i) * P.kv_heads + head;
-    if (4 * lane < D) {
+template <int DT>
+__device__ __forceinline__ void store16(char* out, unsigned lo, unsigned hi, float scale) {  // 8 codes; 16 or 32 bytes
+  const float2 a = decode2(lo), b = decode2(lo >> 16), c = decode2(hi), d = decode2(hi >> 16);
+  const float x[8] = {a.x * scale, a.y * scale, b.x * scale, b.y * scale, c.x * scale, c.y * scale, d.x * scale, d.y * scale};
+  if constexpr (DT == COW_F32) {
+    reinterpret_cast<float4*>(out)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(out)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    unsigned w[4];
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        unsigned codes = 0;
-        float scale = 0.f;
-        if (ok) {
-          scale = P.scales[which][tile];
-          codes = which ? *reinterpret_cast<const unsigned*>(&s_codes[i][4 * lane])
-                        : *reinterpret_cast<const unsigned*>(P.codes[0] + tile * (kPage * D) +
-                                                         (D == 128 ? key_at<128>(slot % kPage, 4 * lane) : (slot % kPage) * D + 4 * lane));
-        }
-        const float2 a = decode2(codes), b = decode2(codes >> 16);
-        st4_rt(P.out[which], row * D + 4 * lane, make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale), P.dtype);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == COW_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned*>(&h);
       }
     }
+    *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kReadThreads) cow_kv8_read_kernel(const __grid_constant__ ReadLaunch P) {
+  constexpr int kSize = DT == COW_F32 ? 4 : 2;
+  constexpr int kVecs = D / 8;        // 8 codes
+  constexpr int kRow = D / 4 + 1;     // words of a row of codes in shared memory, off the bank period
+  __shared__ unsigned s_codes[kReadSlots * kRow];
+  __shared__ int s_slots[kReadSlots];
+  __shared__ int4 s_columns[kReadSlots];  // first slot of the four, entry of it, first and number of the tokens asked for
+  __shared__ int s_count;
+  const int tid = threadIdx.x, head = blockIdx.y;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kReadSlots;
+  const int here = static_cast<int>(min(static_cast<int64_t>(kReadSlots), P.count - base));
+  if (tid < kReadSlots) {
+    int slot = -1;
+    if (tid < here) {
+      slot = P.slots[base + tid];
+      if (slot >= P.pages * kPage) slot = -1;
+    }
+    s_slots[tid] = slot;
+  }
+  auto tile_of = [&](int slot) { return static_cast<int64_t>(slot / kPage) * P.kv_heads + head; };
+  // values: columns, then their words
+  if (tid < kReadSlots) {
+    const int slot = s_slots[tid], prev = __shfl_up_sync(kFull, slot, 1);
+    const bool leads = slot >= 0 && (tid == 0 || slot != prev + 1 || slot % 4 == 0);
+    const unsigned lead = __ballot_sync(kFull, leads), follow = __ballot_sync(kFull, slot >= 0 && !leads);
+    if (leads) {
+      const int first = slot % 4;
+      s_columns[__popc(lead & ((1u << tid) - 1))] =
+          make_int4(slot - first, tid - first, first, __ffs(~(tid < 31 ? follow >> (tid + 1) : 0)));
+    }
+    if (tid == 0) s_count = __popc(lead);
+  }
+  __syncthreads();
+  const int columns = s_count;
+#pragma unroll 4
+  for (int i = tid; i < columns * (D / 4); i += kReadThreads) {
+    const int q = i / columns;
+    const int4 col = s_columns[i - q * columns];
+    const uint8_t* src = P.codes[1] + tile_of(col.x) * (kPage * D) + 4 * q * kPage + col.x % kPage;
+    unsigned w[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) w[d] = __ldg(reinterpret_cast<const unsigned*>(src + d * kPage));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const unsigned lo = __byte_perm(w[0], w[1], t | (4 + t) << 4), hi = __byte_perm(w[2], w[3], t | (4 + t) << 4);
+      if (t >= col.z && t < col.z + col.w) s_codes[(col.y + t) * kRow + q] = __byte_perm(lo, hi, 0x5410);
+    }
+  }
+  // keys, from their rows
+  for (int i = tid; i < here * kVecs; i += kReadThreads) {
+    const int e = i / kVecs, v = i % kVecs, slot = s_slots[e];
+    uint2 w = make_uint2(0, 0);
+    float scale = 0.f;
+    if (slot >= 0) {
+      const int64_t tile = tile_of(slot);
+      w = __ldg(reinterpret_cast<const uint2*>(P.codes[0] + tile * (kPage * D) + key_at<D>(slot % kPage, 8 * v)));
+      scale = P.scales[0][tile];
+    }
+    store16<DT>(P.out[0] + ((base + e) * P.kv_heads + head) * (D * kSize) + v * 8 * kSize, w.x, w.y, scale);
+  }
+  __syncthreads();
+  for (int i = tid; i < here * kVecs; i += kReadThreads) {
+    const int e = i / kVecs, v = i % kVecs, slot = s_slots[e];
+    const bool there = slot >= 0;
+    store16<DT>(P.out[1] + ((base + e) * P.kv_heads + head) * (D * kSize) + v * 8 * kSize, there ? s_codes[e * kRow + 2 * v] : 0,
+                there ? s_codes[e * kRow + 2 * v + 1] : 0, there ? P.scales[1][tile_of(slot)] : 0.f);
   }
 }
 
@@ -1033,6 +1074,14 @@ void launch_store(const StoreLaunch& P, int width, dim3 grid, cudaStream_t strea
   else cow_kv8_store_kernel<DT, 128><<<grid, kStoreThreads, 0, stream>>>(P);
 }
 
+template <int DT>
+void launch_read(const ReadLaunch& P, int width, dim3 grid, cudaStream_t stream) {
+  if (width == 32) cow_kv8_read_kernel<DT, 32><<<grid, kReadThreads, 0, stream>>>(P);
+  else if (width == 64) cow_kv8_read_kernel<DT, 64><<<grid, kReadThreads, 0, stream>>>(P);
+  else if (width == 96) cow_kv8_read_kernel<DT, 96><<<grid, kReadThreads, 0, stream>>>(P);
+  else cow_kv8_read_kernel<DT, 128><<<grid, kReadThreads, 0, stream>>>(P);
+}
+
 using AttendFn = void (*)(const AttendLaunch);
 
 AttendFn attend_fn(int width, bool split) {
@@ -1083,7 +1132,7 @@ int cow_kv8_store(const cow_kv_pages* cache, int32_t layer, const void* keys, in
                 {key_head_stride * size, value_head_stride * size},
                 plan, cache->kv_heads, static_cast<int32_t>(cache->pages)};
   const int64_t pieces = (tokens < tokens / kPage + 2 * cache->requests) ? tokens : tokens / kPage + 2 * cache->requests;
-  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(cache->kv_heads));
+  const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(cache->kv_heads), 2);
   if (dtype == COW_F32) launch_store<COW_F32>(P, cache->width, grid, as_stream(stream));
   else if (dtype == COW_BF16) launch_store<COW_BF16>(P, cache->width, grid, as_stream(stream));
   else launch_store<COW_F16>(P, cache->width, grid, as_stream(stream));
@@ -1103,9 +1152,11 @@ int cow_kv8_read(const cow_kv_pages* cache, int32_t layer, const int32_t* slots,
   ReadLaunch P{{cache->key_codes + bytes, cache->value_codes + bytes},
                {cache->key_scales + tiles, cache->value_scales + tiles},
                {static_cast<char*>(keys), static_cast<char*>(values)},
-               slots, count, cache->kv_heads, static_cast<int32_t>(cache->pages), cache->width, dtype};
+               slots, count, cache->kv_heads, static_cast<int32_t>(cache->pages)};
   const dim3 grid(static_cast<unsigned>((count + kReadSlots - 1) / kReadSlots), static_cast<unsigned>(cache->kv_heads));
-  cow_kv8_read_kernel<<<grid, kStoreThreads, 0, as_stream(stream)>>>(P);
+  if (dtype == COW_F32) launch_read<COW_F32>(P, cache->width, grid, as_stream(stream));
+  else if (dtype == COW_BF16) launch_read<COW_BF16>(P, cache->width, grid, as_stream(stream));
+  else launch_read<COW_F16>(P, cache->width, grid, as_stream(stream));
   return launch_status();
 }
 

@@ -243,8 +243,8 @@ int cow_pages_resize(const cow_kv_pages* cache, const int32_t* targets, int64_t 
   if (!resident_blocks(reinterpret_cast<const void*>(cow_pages_resize_kernel), kResizeThreads,
                        sizeof(int) * (6 * COW_MAX_REQUESTS + 4)))
     return COW_ERR_CUDA;
-  // a block for each 2,048 tokens of the maps, one for each SM at most
-  const int grid = grid_for(tokens, kResizeThreads * kTokensPerThread, 148);
+  // a block for each 2,048 tokens of the maps and 2,048 table entries (pages may move without tokens), one for each SM at most
+  const int grid = grid_for(tokens + requests * cache->max_blocks, kResizeThreads * kTokensPerThread, 148);
   cow_pages_resize_kernel<<<grid, kResizeThreads, smem, as_stream(stream)>>>(P);
   return launch_status();
 }

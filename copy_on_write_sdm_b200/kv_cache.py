@@ -122,29 +122,35 @@ class PagePlan:
     offset`` in the cache, place in the request; -1 past the new tokens), all int32 on
     the device, and ``pieces`` (the new tokens page by page) for ``store``."""
 
-    __slots__ = ("cache", "epoch", "requests", "tokens", "buffer", "_at")
+    __slots__ = ("cache", "epoch", "requests", "tokens", "buffer", "_views")
 
     def __init__(self, cache: "PagedKVCache", epoch: int, tokens: int, buffer: torch.Tensor) -> None:
         self.cache, self.epoch, self.tokens, self.buffer = cache, epoch, tokens, buffer
         self.requests = cache.requests
-        self._at = buffer.numel() - (self.requests + 1 + 2 * tokens)
+        self._views = None
+
+    def _parts(self) -> tuple[torch.Tensor, ...]:
+        if self._views is None:
+            tail = (self.requests + 1, self.tokens, self.tokens)
+            self._views = self.buffer.split_with_sizes((4, self.buffer.numel() - 4 - sum(tail), *tail))
+        return self._views
 
     @property
     def starts(self) -> torch.Tensor:
-        return self.buffer[self._at:self._at + self.requests + 1]
+        return self._parts()[2]
 
     @property
     def slots(self) -> torch.Tensor:
-        return self.buffer[self._at + self.requests + 1:self._at + self.requests + 1 + self.tokens]
+        return self._parts()[3]
 
     @property
     def positions(self) -> torch.Tensor:
-        return self.buffer[self.buffer.numel() - self.tokens:]
+        return self._parts()[4]
 
     @property
     def pieces(self) -> torch.Tensor:
         """``[max pieces, 4]``: first packed token, tokens, page, offset; the first ``buffer[0]`` are set."""
-        return self.buffer[4:self._at].view(-1, 4)
+        return self._parts()[1].view(-1, 4)
 
 
 @dataclass(frozen=True, eq=False)
