@@ -2,10 +2,10 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale * q_i . k_j - m_i),   j <= i in i's own sequence
 //
-// A tile is kRows rows of one key head: neighbouring tokens times the key head's query heads, row =
+// A tile is some rows of one key head: neighbouring tokens times the key head's query heads, row =
 // token * group + head, so that a group shares every key it reads and short prompts still fill
-// their rows.  Keys pass in tiles of 64; maximum, sum and output of the running softmax stay in
-// registers.  Tiles run in the order of their work, longest first, over all sequences
+// their rows.  Keys pass in tiles; maximum, sum and output of the running softmax stay on the SM.
+// Tiles run in the order of their work, longest first, over all sequences
 // together: the tile at place l of its sequence reads l + 1 tiles' keys, so the tiles of place l
 // are one for each sequence that has more than l, and one is found by a search
 // over l with no table to build.
@@ -109,145 +109,319 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // --------------------------------------------------------------------------
-// f32 arithmetic
+// f32
 // --------------------------------------------------------------------------
 //
-// 64 rows against 64 keys at a time, 256 threads, each 4 x 4 scores and 4 rows x width / 16 of the output.
+// Each operand is held as two f16 parts, hi and lo, after a scale by a power of two that brings its row's
+// (queries) or tile's (keys, values) largest magnitude to [2^14, 2^15): 22 bits of it, and three of the four
+// part products on the f16 matrix instructions with f32 sums, lo * lo being below the others' rounding.  That
+// is f32's accuracy to a few units at a third of the f16 rate, several times what the f32 pipe
+// gives.  A tile of 64 keys is split once for the whole block.  Probabilities are split the same way, from
+// 2^14 down; value scales ride on the factor that rescales the output when a maximum moves.
+// Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
+// the end to the rows that see them.
 
-constexpr int kRows = 64;
 constexpr int kKeys = 64;
-constexpr int kThreads = 256;
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
-  constexpr int kStride = D + 4;
-  constexpr int kCols = D / 16;
-  extern __shared__ __align__(16) float smem_f[];
-  float* s_q = smem_f;                     // [kRows][kStride]
-  float* s_k = s_q + kRows * kStride;      // [kKeys][kStride]
-  float* s_v = s_k + kKeys * kStride;      // [kKeys][kStride]
-  float* s_p = s_v + kKeys * kStride;      // [kRows][kKeys + 4]
+struct F32Shape {
+  static constexpr int kWarps = D > 64 ? 8 : 4;  // 16 rows each
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kRows = 16 * kWarps;
+  static constexpr int kStride = D + 8;          // halves of a row in shared memory: rows apart by an odd number of 16 bytes
+  static constexpr int kVecs = kKeys * D / 4 / kThreads;  // 16-byte words of a tile per thread
+  static constexpr int kBytes = 2 * (2 * kRows + 4 * kKeys) * kStride;
+};
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
+// The exponent of the scale that brings `most` (finite, >= 0) to [2^14, 2^15), as far as both are normal.
+__device__ __forceinline__ int split_exponent(float most) { return min(max(14 - ((__float_as_int(most) >> 23) - 127), -113), 100); }
+
+__device__ __forceinline__ unsigned pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+// hi and lo parts of a and b; lo is 0 where hi is not finite
+__device__ __forceinline__ uint2 split2(float a, float b) {
+  const unsigned hi = pack_half2(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return make_uint2(hi, pack_half2(fabsf(h.x) < INFINITY ? a - h.x : 0.f, fabsf(h.y) < INFINITY ? b - h.y : 0.f));
+}
+__device__ __forceinline__ void mma_f16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void load_matrices(unsigned* r, const __half* at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(at))
+               : "memory");
+}
+__device__ __forceinline__ void load_matrices_turned(unsigned* r, const __half* at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_addr(at))
+               : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : 3) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
+  using S = F32Shape<D>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __half* s_q = reinterpret_cast<__half*>(smem_raw);       // [2][kRows][kStride] hi, lo
+  __half* s_k = s_q + 2 * S::kRows * S::kStride;           // [2][kKeys][kStride]
+  __half* s_v = s_k + 2 * kKeys * S::kStride;              // [2][kKeys][kStride]
   __shared__ Tile s_tile;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int group = P.group, tile_tokens = kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
-  if (tid < 32) {
+  __shared__ int2 s_most[S::kWarps];
+  __shared__ int s_bad;
+  __shared__ int s_row[S::kRows];                          // scale exponents of the query rows
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int group = P.group, tile_tokens = S::kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
+  const float* Q = static_cast<const float*>(P.q);
+  const float* K = static_cast<const float*>(P.k) + kv_head * P.k_head;
+  const float* V = static_cast<const float*>(P.v) + kv_head * P.v_head;
+  if (warp == 0) {
     TileFinder finder;
     finder.begin(P, tile_tokens);
     const Tile t = finder.find(P, tile_tokens, blockIdx.x / P.kv_heads);
-    if (tid == 0) s_tile = t;
+    if (lane == 0) {
+      s_tile = t;
+      s_bad = 0;
+    }
   }
   __syncthreads();
   const Tile t = s_tile;
   if (t.count == 0) return;
   const int here = min(tile_tokens, t.count - t.first);  // tokens of this tile
+  const int last = t.first + here;                       // keys 0 .. last - 1
 
-  for (int i = tid; i < kRows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), d = 4 * (i % (D / 4)), token = r / group, h = r % group;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (token < here && d < W)
-      x = ld4_rt(P.q, (t.begin + t.first + token) * P.q_token + (static_cast<int64_t>(kv_head) * group + h) * P.q_head + d, P.dtype);
-    *reinterpret_cast<float4*>(s_q + r * kStride + d) = x;
-  }
-  float o[4][kCols], m[4], l[4];
+  float4 k[S::kVecs], v[S::kVecs];
+  auto load = [&](int j0) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kCols; ++j) o[i][j] = 0.f;
-  }
-  const int last = t.first + here;  // keys 0 .. last - 1
-  for (int j0 = 0; j0 < last; j0 += kKeys) {
-    __syncthreads();
-    for (int i = tid; i < kKeys * (D / 4); i += kThreads) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int i = 0; i < S::kVecs; ++i) {
+      const int n = tid + i * S::kThreads, r = n / (D / 4), d = 4 * (n % (D / 4));
+      k[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (j0 + r < last && d < W) {
         const int64_t token = t.begin + j0 + r;
-        a = ld4_rt(P.k, token * P.k_token + kv_head * P.k_head + d, P.dtype);
-        b = ld4_rt(P.v, token * P.v_token + kv_head * P.v_head + d, P.dtype);
+        k[i] = __ldg(reinterpret_cast<const float4*>(K + token * P.k_token + d));
+        v[i] = __ldg(reinterpret_cast<const float4*>(V + token * P.v_token + d));
       }
-      *reinterpret_cast<float4*>(s_k + r * kStride + d) = a;
-      *reinterpret_cast<float4*>(s_v + r * kStride + d) = b;
+    }
+  };
+  // queries: a warp's own 16 rows, kLanes lanes to a row, all loads under way before the first is used
+  {
+    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kTurns = 16 / kAtOnce;
+    const int sub = lane / kLanes, d = 4 * (lane % kLanes);
+    float4 x[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int r = 16 * warp + i * kAtOnce + sub, token = r / group;
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (token < here && d < W)
+        x[i] = __ldg(reinterpret_cast<const float4*>(Q + (t.begin + t.first + token) * P.q_token +
+                                                     (static_cast<int64_t>(kv_head) * group + r % group) * P.q_head + d));
+    }
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int r = 16 * warp + i * kAtOnce + sub;
+      float most = 0.f;
+      const float e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (fabsf(e[u]) < INFINITY) most = fmaxf(most, fabsf(e[u]));
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+      const int scale = split_exponent(most);
+      const float up = pow2(scale);
+      if (d == 0) s_row[r] = scale;
+      const uint2 a = split2(x[i].x * up, x[i].y * up), b = split2(x[i].z * up, x[i].w * up);
+      *reinterpret_cast<uint2*>(s_q + r * S::kStride + d) = make_uint2(a.x, b.x);
+      *reinterpret_cast<uint2*>(s_q + (S::kRows + r) * S::kStride + d) = make_uint2(a.y, b.y);
+    }
+  }
+  load(0);
+  __syncwarp();
+  const int row0 = 16 * warp + g;  // this lane's rows: row0 and row0 + 8
+  const int query0 = t.first + row0 / group, query1 = t.first + (row0 + 8) / group;  // their places in the sequence
+  const int sq0 = s_row[row0], sq1 = s_row[row0 + 8];
+
+  float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  int unit = 0;  // the output is held times 2^(unit + 14)
+
+  for (int j0 = 0; j0 < last; j0 += kKeys) {
+    // the tile's scales, over the block
+    float mk = 0.f, mv = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < S::kVecs; ++i) {
+      const float a[4] = {k[i].x, k[i].y, k[i].z, k[i].w}, b[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (fabsf(a[u]) < INFINITY) mk = fmaxf(mk, fabsf(a[u]));
+        if (fabsf(b[u]) < INFINITY) mv = fmaxf(mv, fabsf(b[u]));
+        else bad = true;
+      }
+    }
+    const int2 found = make_int2(__reduce_max_sync(kFull, __float_as_int(mk)), __reduce_max_sync(kFull, __float_as_int(mv)));
+    if (lane == 0) s_most[warp] = found;
+    if (bad) s_bad = 1;
+    __syncthreads();  // also: the last tile is used up
+    int2 most = s_most[0];
+#pragma unroll
+    for (int w = 1; w < S::kWarps; ++w) most = make_int2(max(most.x, s_most[w].x), max(most.y, s_most[w].y));
+    const int ek = split_exponent(__int_as_float(most.x));
+    const int ev = most.y > 0 ? split_exponent(__int_as_float(most.y)) : unit;
+    const float uk = pow2(ek), uv = pow2(ev);
+#pragma unroll
+    for (int i = 0; i < S::kVecs; ++i) {
+      const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
+      uint2 a = split2(k[i].x * uk, k[i].y * uk), b = split2(k[i].z * uk, k[i].w * uk);
+      *reinterpret_cast<uint2*>(s_k + at) = make_uint2(a.x, b.x);
+      *reinterpret_cast<uint2*>(s_k + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
+      auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
+      a = split2(finite(v[i].x) * uv, finite(v[i].y) * uv);
+      b = split2(finite(v[i].z) * uv, finite(v[i].w) * uv);
+      *reinterpret_cast<uint2*>(s_v + at) = make_uint2(a.x, b.x);
+      *reinterpret_cast<uint2*>(s_v + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
     }
     __syncthreads();
-    float s[4][4] = {};
-#pragma unroll 4
-    for (int d = 0; d < D; d += 4) {
-      float4 a[4], b[4];
+    if (j0 + kKeys < last) load(j0 + kKeys);
+
+    // scores: 16 rows x 64 keys
+    float s[8][4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(s_q + (4 * ty + i) * kStride + d);
+    for (int d = 0; d < D; d += 16) {
+      if (d >= W) break;
+      unsigned qh[4], ql[4];
+      const __half* at = s_q + (16 * warp + (lane & 15)) * S::kStride + d + (lane >> 4) * 8;
+      load_matrices(qh, at);
+      load_matrices(ql, at + S::kRows * S::kStride);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(s_k + (tx + 16 * j) * kStride + d);
+      for (int n = 0; n < 4; n += 2) {  // 32 keys: four sums take turns, as each product waits for the last of its sum
+        unsigned kh[8], kl[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
-          s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
-          s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
-          s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+        for (int x = 0; x < 2; ++x) {
+          const __half* b = s_k + (16 * (n + x) + (lane & 7) + (lane >> 4) * 8) * S::kStride + d + (lane >> 3 & 1) * 8;
+          load_matrices(kh + 4 * x, b);
+          load_matrices(kl + 4 * x, b + kKeys * S::kStride);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int query = t.first + (4 * ty + i) / group;  // its place in the sequence
-      float big = -INFINITY;
+        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], ql, kh[2 * x], kh[2 * x + 1]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = j0 + tx + 16 * j <= query ? s[i][j] * P.scale_log2 : -INFINITY;
-        big = fmaxf(big, s[i][j]);
-      }
+        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], qh, kl[2 * x], kl[2 * x + 1]);
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, x));
-      const float n = fmaxf(m[i], big), base = n == -INFINITY ? 0.f : n;
-      const float a = exp2_fast(m[i] - base);
-      m[i] = n;
-      l[i] *= a;
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) o[i][j] *= a;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = exp2_fast(s[i][j] - base);
-        l[i] += e;
-        s_p[(4 * ty + i) * (kKeys + 4) + tx + 16 * j] = e;
+        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], qh, kh[2 * x], kh[2 * x + 1]);
       }
     }
-    __syncwarp();  // a row's 16 threads are of one warp
-    const int keys = min(kKeys, last - j0);
-    for (int j = 0; j < keys; ++j) {
-      float p[4];
+    // softmax: columns 8 n + 2 c and the next of rows row0, row0 + 8
+    const float f0 = pow2(min(max(-sq0 - ek, -126), 127)) * P.scale_log2, f1 = pow2(min(max(-sq1 - ek, -126), 127)) * P.scale_log2;
+    float big0 = -INFINITY, big1 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = s_p[(4 * ty + i) * (kKeys + 4) + j];
-        // a key after the query has no part in it, whatever its value (0 * inf is not 0)
-        if (j0 + j > t.first + (4 * ty + i) / group) p[i] = 0.f;
+    for (int n = 0; n < 8; ++n) {
+      const int key = j0 + 8 * n + 2 * c;
+      s[n][0] = key <= query0 ? s[n][0] * f0 : -INFINITY;
+      s[n][1] = key + 1 <= query0 ? s[n][1] * f0 : -INFINITY;
+      s[n][2] = key <= query1 ? s[n][2] * f1 : -INFINITY;
+      s[n][3] = key + 1 <= query1 ? s[n][3] * f1 : -INFINITY;
+      big0 = fmaxf(big0, fmaxf(s[n][0], s[n][1]));
+      big1 = fmaxf(big1, fmaxf(s[n][2], s[n][3]));
+    }
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, x));
+      big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, x));
+    }
+    const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
+    const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;  // all -inf so far: weights 0
+    float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
+    m0 = n0;
+    m1 = n1;
+    l0 *= a0;
+    l1 *= a1;
+    // The output follows the tile's value scale; a tile 2^64 below the others keeps theirs and its weights
+    // shrink instead, so no factor overflows.
+    if (j0 == 0) unit = ev;
+    int step = ev - unit;
+    float shrink = 1.f;
+    if (step > 64) {
+      shrink = pow2(max(-step, -126));
+      step = 0;
+    }
+    unit += step;
+    const float follow = step < -126 ? 0.f : pow2(step);
+    a0 *= follow;
+    a1 *= follow;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      o[i][0] *= a0;
+      o[i][1] *= a0;
+      o[i][2] *= a1;
+      o[i][3] *= a1;
+    }
+    constexpr float kUp = 16384.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {  // 16 keys
+      unsigned ph[4], pl[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float e0 = exp2_fast(s[2 * n + x][0] - b0), e1 = exp2_fast(s[2 * n + x][1] - b0);
+        const float e2 = exp2_fast(s[2 * n + x][2] - b1), e3 = exp2_fast(s[2 * n + x][3] - b1);
+        l0 += e0 + e1;
+        l1 += e2 + e3;
+        const uint2 u = split2(e0 * shrink * kUp, e1 * shrink * kUp), w = split2(e2 * shrink * kUp, e3 * shrink * kUp);
+        ph[2 * x] = u.x;
+        ph[2 * x + 1] = w.x;
+        pl[2 * x] = u.y;
+        pl[2 * x + 1] = w.y;
       }
 #pragma unroll
-      for (int x = 0; x < kCols; ++x) {
-        const float v = s_v[j * kStride + tx + 16 * x];
+      for (int d = 0; d < D; d += 32) {
+        if (d >= W) break;
+        unsigned vh[8], vl[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j0 + j <= t.first + (4 * ty + i) / group) o[i][x] = fmaf(p[i], v, o[i][x]);
+        for (int x = 0; x < 2; ++x) {
+          const __half* b = s_v + (16 * n + (lane & 15)) * S::kStride + d + 16 * x + (lane >> 4) * 8;
+          load_matrices_turned(vh + 4 * x, b);
+          load_matrices_turned(vl + 4 * x, b + kKeys * S::kStride);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], pl, vh[2 * x], vh[2 * x + 1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], ph, vl[2 * x], vl[2 * x + 1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], ph, vh[2 * x], vh[2 * x + 1]);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int x = 1; x < 4; x <<= 1) {
+    l0 += __shfl_xor_sync(kFull, l0, x);
+    l1 += __shfl_xor_sync(kFull, l1, x);
+  }
+  const float down = pow2(min(max(-unit - 14, -126), 127));
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(kFull, l[i], x);
-    const int r = 4 * ty + i, token = r / group, h = r % group;
+  for (int half = 0; half < 2; ++half) {
+    const int r = row0 + 8 * half, token = r / group, query = half ? query1 : query0;
     if (token >= here || r >= tile_tokens * group) continue;
-    const float inv = 1.f / l[i];
-    const int64_t row = (static_cast<int64_t>(t.begin + t.first + token) * P.heads + static_cast<int64_t>(kv_head) * group + h) * W;
+    const float inv = 1.f / (half ? l1 : l0);
+    float* out = static_cast<float*>(P.out) +
+                 (static_cast<int64_t>(t.begin + query) * P.heads + static_cast<int64_t>(kv_head) * group + r % group) * W;
 #pragma unroll
-    for (int x = 0; x < kCols; ++x) {
-      const int d = tx + 16 * x;
+    for (int i = 0; i < D / 8; ++i) {
+      const int d = 8 * i + 2 * c;
       if (d >= W) continue;
-      const float y = o[i][x] * inv;
-      if (P.dtype == COW_F32) static_cast<float*>(P.out)[row + d] = y;
-      else if (P.dtype == COW_BF16) static_cast<__nv_bfloat16*>(P.out)[row + d] = __float2bfloat16_rn(y);
-      else static_cast<__half*>(P.out)[row + d] = __float2half_rn(y);
+      float2 y = make_float2(o[i][2 * half] * down * inv, o[i][2 * half + 1] * down * inv);
+      if (s_bad) {  // seen values that are not finite
+        for (int j = 0; j <= query; ++j) {
+          const float2 x = __ldg(reinterpret_cast<const float2*>(V + (t.begin + j) * P.v_token + d));
+          if (!(fabsf(x.x) < INFINITY)) y.x += x.x;
+          if (!(fabsf(x.y) < INFINITY)) y.y += x.y;
+        }
+      }
+      *reinterpret_cast<float2*>(out + d) = y;
     }
   }
 }
@@ -961,19 +1135,18 @@ int prompt_tc(const PromptLaunch& P, cudaStream_t stream) {
 }
 
 template <int D>
-int launch_f32(const PromptLaunch& P, unsigned blocks, cudaStream_t stream) {
-  constexpr size_t kBytes = sizeof(float) * ((kRows + 2 * kKeys) * (D + 4) + kRows * (kKeys + 4));
-  if (!resident_blocks(reinterpret_cast<const void*>(cow_prompt_f32_kernel<D>), kThreads, kBytes)) return COW_ERR_CUDA;
-  cow_prompt_f32_kernel<D><<<blocks, kThreads, kBytes, stream>>>(P);
+int launch_f32(const PromptLaunch& P, cudaStream_t stream) {
+  using S = F32Shape<D>;
+  if (!resident_blocks(reinterpret_cast<const void*>(cow_prompt_f32_kernel<D>), S::kThreads, S::kBytes)) return COW_ERR_CUDA;
+  // every sequence adds at most one tile that is not full
+  const int64_t tiles = P.tokens / (S::kRows / P.group) + (P.sequences < P.tokens ? P.sequences : P.tokens);
+  cow_prompt_f32_kernel<D><<<static_cast<unsigned>(tiles * P.kv_heads), S::kThreads, S::kBytes, stream>>>(P);
   return launch_status();
 }
 
 int prompt_f32(const PromptLaunch& P, cudaStream_t stream) {
-  // every sequence adds at most one tile that is not full
-  const int64_t tiles = P.tokens / (kRows / P.group) + (P.sequences < P.tokens ? P.sequences : P.tokens);
-  const unsigned blocks = static_cast<unsigned>(tiles * P.kv_heads);
-  if (P.width <= 32) return launch_f32<32>(P, blocks, stream);
-  return P.width <= 64 ? launch_f32<64>(P, blocks, stream) : launch_f32<128>(P, blocks, stream);
+  if (P.width <= 32) return launch_f32<32>(P, stream);
+  return P.width <= 64 ? launch_f32<64>(P, stream) : launch_f32<128>(P, stream);
 }
 
 bool rows_ok(const void* p, int64_t s0, int64_t s1, int dtype) {
@@ -996,7 +1169,7 @@ int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_
       sequences >= (int64_t{1} << 30))
     return COW_ERR_UNSUPPORTED;
   if (sequences == 0 || tokens == 0) return COW_OK;
-  if ((tokens / (kRows / (heads / kv_heads)) + (sequences < tokens ? sequences : tokens)) * kv_heads >= (int64_t{1} << 31))
+  if ((tokens / (kMaxGroup / (heads / kv_heads)) + (sequences < tokens ? sequences : tokens)) * kv_heads >= (int64_t{1} << 31))
     return COW_ERR_UNSUPPORTED;  // more blocks than one launch has
   if (!rows_ok(queries, query_token_stride, query_head_stride, dtype) ||
       !rows_ok(keys, key_token_stride, key_head_stride, dtype) ||
