@@ -315,11 +315,13 @@ class PagedKVCache:
         return out
 
     def new_workspace(self, heads: int) -> torch.Tensor:
-        """A zero-filled workspace of ``attend`` for ``heads`` query heads."""
+        """A workspace of ``attend`` for ``heads`` query heads."""
         need = _lib.load().cow_kv8_attend_workspace_bytes(self._at, heads)
         if need < 0:
             raise ValueError("heads must be a multiple of kv_heads")
-        return torch.zeros(need, dtype=torch.uint8, device=self.device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        workspace[:16].zero_()
+        return workspace
 
     # ---- lifecycle
 
@@ -336,7 +338,9 @@ class PagedKVCache:
         tables[:keep.shape[0]] = self.block_tables[keep]
         lengths[:keep.shape[0]] = self.lengths[keep]
         self._epoch[0] += 1  # plans made for the old slots are over
-        return replace(self, block_tables=tables, lengths=lengths)
+        cache = replace(self, block_tables=tables, lengths=lengths)
+        object.__setattr__(cache, "_workspaces", self._workspaces)  # their size does not depend on the requests
+        return cache
 
     def validate_invariants(self) -> None:
         """Raise on a device error, or where live and free pages do not partition the pool (synchronises)."""

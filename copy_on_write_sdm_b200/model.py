@@ -17,9 +17,11 @@ import torch.nn.functional as F
 from torch import nn
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
+from .kv_cache import prompt_attention
 from .sdm import SparseDeltaMemory
 
 if TYPE_CHECKING:
+    from .kv_cache import PagedKVCache, PagePlan
     from .inference import FaithfulSDMDecodeState
 
 
@@ -40,24 +42,51 @@ class ResidualMLP(nn.Module):
 
 
 class CausalSelfAttention(nn.Module):
-    """Multi-head causal attention with a fixed-capacity K/V cache (reference model.py:47-190)."""
+    """Multi-head causal attention with a fixed-capacity K/V cache (reference model.py:47-190).
 
-    def __init__(self, width: int, heads: int, *, dropout: float = 0.0) -> None:
+    ``kv_heads`` (all heads by default, as in the reference) lets neighbouring query heads
+    share a key and value head.  ``prefill_packed`` / ``decode_packed`` serve requests of
+    different lengths over a paged 8-bit cache (``PagedKVCache``).
+    """
+
+    def __init__(self, width: int, heads: int, *, kv_heads: int | None = None, dropout: float = 0.0) -> None:
         super().__init__()
         if width <= 0 or heads <= 0 or width % heads:
             raise ValueError("width must be positive and divisible by heads")
         self.width, self.heads, self.head_width, self.dropout = width, heads, width // heads, dropout
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if self.kv_heads <= 0 or heads % self.kv_heads:
+            raise ValueError("heads must be divisible by kv_heads")
         self.norm = nn.LayerNorm(width)
-        self.qkv = nn.Linear(width, 3 * width, bias=False)
+        self.qkv = nn.Linear(width, width + 2 * self.kv_heads * self.head_width, bias=False)
         self.output = nn.Linear(width, width, bias=False)
 
     def project_qkv(self, tokens: torch.Tensor):
         batch, time, _ = tokens.shape
-        qkv = self.qkv(self.norm(tokens)).reshape(batch, time, 3, self.heads, self.head_width)
-        q, k, v = (qkv[:, :, i].transpose(1, 2).contiguous() for i in range(3))
+        qkv = self.qkv(self.norm(tokens)).reshape(batch, time, self.heads + 2 * self.kv_heads, self.head_width)
+        q, k, v = (t.transpose(1, 2).contiguous() for t in qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=2))
         return q, k, v
 
+    def _project_packed(self, tokens: torch.Tensor):
+        qkv = self.qkv(self.norm(tokens)).view(tokens.shape[0], self.heads + 2 * self.kv_heads, self.head_width)
+        return qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
+
+    def prefill_packed(self, tokens: torch.Tensor, plan: "PagePlan", cache: "PagedKVCache", *, layer: int) -> torch.Tensor:
+        """Whole prompts of a plan's requests, packed ``[tokens, width]``; their K/V go to the cache."""
+        q, k, v = self._project_packed(tokens)
+        attended = prompt_attention(q, k, v, plan.starts)
+        cache.store(k, v, plan, layer=layer)
+        return self.output(attended.view(-1, self.width))
+
+    def decode_packed(self, tokens: torch.Tensor, plan: "PagePlan", cache: "PagedKVCache", *, layer: int) -> torch.Tensor:
+        """One token of every request, ``[requests, width]``, over the cache that it joins."""
+        q, k, v = self._project_packed(tokens)
+        cache.store(k, v, plan, layer=layer)
+        return self.output(cache.attend(q, layer=layer).view(-1, self.width))
+
     def _sdpa(self, q, k, v, *, causal: bool, mask=None) -> torch.Tensor:
+        if self.kv_heads != self.heads:
+            k, v = (t.repeat_interleave(self.heads // self.kv_heads, dim=1) for t in (k, v))
         # Flash kernels for 16-bit activations, the exact math kernel for fp32.
         if q.is_cuda:
             backend = SDPBackend.FLASH_ATTENTION if (q.dtype in (torch.float16, torch.bfloat16) and mask is None) \
@@ -102,9 +131,10 @@ class CausalSelfAttention(nn.Module):
 
 
 class DenseAttentionBlock(nn.Module):
-    def __init__(self, width: int, heads: int, *, mlp_expansion: float = 4.0, dropout: float = 0.0) -> None:
+    def __init__(self, width: int, heads: int, *, kv_heads: int | None = None, mlp_expansion: float = 4.0,
+                 dropout: float = 0.0) -> None:
         super().__init__()
-        self.attention = CausalSelfAttention(width, heads, dropout=dropout)
+        self.attention = CausalSelfAttention(width, heads, kv_heads=kv_heads, dropout=dropout)
         self.mlp = ResidualMLP(width, expansion=mlp_expansion, dropout=dropout)
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
@@ -127,6 +157,8 @@ class DenseAttentionBlock(nn.Module):
         if not (tokens.is_cuda and tokens.dtype == key_cache.dtype == value_cache.dtype == torch.float32):
             return False
         if self.training or tokens.ndim != 3 or tokens.shape[1] != 1:
+            return False
+        if att.kv_heads != att.heads:
             return False
         if not (key_cache.is_contiguous() and value_cache.is_contiguous() and key_cache.shape == value_cache.shape
                 and key_cache.shape[:2] == (tokens.shape[0], att.heads) and key_cache.shape[3] == att.head_width):
@@ -191,13 +223,14 @@ class SDMDecoderStack(nn.Module):
     """Layout string of "A" (dense attention) and "B" (SDM) physical layers (reference model.py:214-325)."""
 
     def __init__(self, *, layout: str, width: int, heads: int, slots: int, reads: int, writes: int,
-                 memory_heads: int = 1, mlp_expansion: float = 4.0, dropout: float = 0.0) -> None:
+                 memory_heads: int = 1, mlp_expansion: float = 4.0, dropout: float = 0.0,
+                 kv_heads: int | None = None) -> None:
         super().__init__()
         if not layout or any(kind not in "AB" for kind in layout):
             raise ValueError("layout must contain only A and B")
         self.layout, self.width, self.heads = layout, width, heads
         self.attention_layers = nn.ModuleDict({
-            str(i): DenseAttentionBlock(width, heads, mlp_expansion=mlp_expansion, dropout=dropout)
+            str(i): DenseAttentionBlock(width, heads, kv_heads=kv_heads, mlp_expansion=mlp_expansion, dropout=dropout)
             for i, kind in enumerate(layout) if kind == "A"})
         self.sdm_layers = nn.ModuleDict({
             str(i): SparseDeltaMemory(width, slots=slots, reads=reads, writes=writes, memory_heads=memory_heads)
@@ -236,14 +269,15 @@ class LanguageModel(nn.Module):
 
     def __init__(self, *, vocab_size: int, maximum_sequence_length: int, layout: str, width: int, heads: int,
                  slots: int, reads: int, writes: int, memory_heads: int = 1, mlp_expansion: float = 4.0,
-                 activation_dtype: torch.dtype = torch.bfloat16) -> None:
+                 activation_dtype: torch.dtype = torch.bfloat16, kv_heads: int | None = None) -> None:
         super().__init__()
         self.maximum_sequence_length = maximum_sequence_length
         self.activation_dtype = activation_dtype
         self.token_embedding = nn.Embedding(vocab_size, width)
         self.position_embedding = nn.Embedding(maximum_sequence_length, width)
         self.stack = SDMDecoderStack(layout=layout, width=width, heads=heads, slots=slots, reads=reads,
-                                     writes=writes, memory_heads=memory_heads, mlp_expansion=mlp_expansion)
+                                     writes=writes, memory_heads=memory_heads, mlp_expansion=mlp_expansion,
+                                     kv_heads=kv_heads)
         self.final_norm = nn.LayerNorm(width)
         self.output = nn.Linear(width, vocab_size, bias=False)
 
