@@ -36,6 +36,12 @@ __device__ __forceinline__ int2 sequence_of(const PromptLaunch& P, int b) {
   return make_int2(begin, end - begin);
 }
 
+// The lane of the (n + 1)-th set bit of `has` (the same in the whole warp, n below its bits' number).
+__device__ __forceinline__ int nth_lane(unsigned has, int n) {
+  const int lane = threadIdx.x & 31;
+  return __ffs(__ballot_sync(kFull, (has >> lane & 1) && __popc(has & ((1u << lane) - 1)) == n)) - 1;
+}
+
 struct Tile {
   int begin, count, first;  // its sequence, and its first token in it; count 0: none left
 };
@@ -85,12 +91,12 @@ struct TileFinder {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const unsigned has = __ballot_sync(kFull, held[i] > lo);
-      if (b < 0 && rank < __popc(has)) b = 32 * i + __fns(has, 0, rank + 1);
+      if (b < 0 && rank < __popc(has)) b = 32 * i + nth_lane(has, rank);
       rank -= __popc(has);
     }
     for (int base = 32 * kHeld; b < 0 && base < P.sequences; base += 32) {
       const unsigned has = __ballot_sync(kFull, tiles_of(P, tile_tokens, base + lane) > lo);
-      if (rank < __popc(has)) b = base + __fns(has, 0, rank + 1);
+      if (rank < __popc(has)) b = base + nth_lane(has, rank);
       rank -= __popc(has);
     }
     if (b < 0) return t;
@@ -466,8 +472,9 @@ struct TcShape {
   static constexpr int kPartBytes = 128 * 128;                  // 128 rows of one part
   static constexpr int kTileBytes = kParts * kPartBytes;
   static constexpr int kSlots = DP > 64 ? 4 : 8;                // ring of K and V tiles
-  static constexpr int kPoly = DP > 64 ? 2 : 3;                 // of 8 pairs of weights, those from the polynomial
-  static constexpr int kBytes = (2 + kSlots) * kTileBytes + 1024;
+  static constexpr int kPoly = 2;                               // of 8 pairs of weights, those from the polynomial
+  static constexpr int kStage = 16 * 1024;                      // 1 KB for each softmax warp: outputs on their way to rows
+  static constexpr int kBytes = (2 + kSlots) * kTileBytes + kStage + 1024;
 };
 
 struct TcLaunch {
@@ -511,6 +518,19 @@ __device__ __forceinline__ unsigned long long nanoseconds() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
+}
+
+// A wait that was not over at once, out of line: the roles' code has to stay small for the instruction caches.
+__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* abort) {
+  const unsigned long long since = nanoseconds();
+  while (!mbar_wait(bar, parity, 64)) {
+    if (*abort) return false;
+    if (nanoseconds() - since > kTcPatience) {
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
 }
 
 // One thread of a converged warp, known to the compiler to be one.
@@ -662,6 +682,23 @@ __device__ __forceinline__ unsigned zero_times(unsigned w, unsigned sum) {
   return r;
 }
 
+// Adds to a row's output the values of tokens first..last that are not finite: those of every 32 columns of
+// two, from column `from` on.
+template <int DT>
+__device__ __noinline__ void add_nonfinite(const PromptLaunch& P, int first, int last, int kv_head, uint16_t* out, int from) {
+  auto value = [](uint16_t u) {
+    return DT == COW_BF16 ? __uint_as_float(static_cast<unsigned>(u) << 16) : __half2float(*reinterpret_cast<const __half*>(&u));
+  };
+  for (int d = from; d < P.width; d += d % 32 == 31 ? 33 : 1) {
+    float sum = value(out[d]);
+    for (int j = first; j <= last; ++j) {
+      const float f = value(static_cast<const uint16_t*>(P.v)[j * P.v_token + kv_head * P.v_head + d]);
+      if (!(fabsf(f) < INFINITY)) sum += f;
+    }
+    out[d] = static_cast<uint16_t>(pack2<DT>(sum, 0.f));
+  }
+}
+
 template <int DT, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __grid_constant__ TcLaunch L) {
   using S = TcShape<DP>;
@@ -678,6 +715,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;  // tiles A and B
   uint8_t* s_ring = smem + 2 * S::kTileBytes;
+  uint8_t* s_stage = s_ring + S::kSlots * S::kTileBytes;
 
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
@@ -707,19 +745,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const unsigned tmem = s_tmem;
-  volatile int* abort = &s_abort;
-  auto wait = [&](uint64_t* bar, unsigned parity) {
-    if (mbar_wait(bar, parity, 4)) return true;
-    const unsigned long long since = nanoseconds();
-    while (!mbar_wait(bar, parity, 64)) {
-      if (*abort) return false;
-      if (nanoseconds() - since > kTcPatience) {
-        *abort = 1;
-        return false;
-      }
-    }
-    return true;
-  };
+  auto wait = [&](uint64_t* bar, unsigned parity) { return mbar_wait(bar, parity, 1) || wait_long(bar, parity, &s_abort); };
   // the i-th of this block's tiles; false: none left, or a wait gave up
   auto next_tile = [&](int i, TcTile& t) {
     if (!wait(&bars.tile_full[i & 1], (i >> 1) & 1)) return false;
@@ -923,7 +949,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   } else if (warp < 16) {
     // ---- softmax
     const int x = warp >> 3, half = (warp >> 2) & 1;  // this thread's half of the keys
-    const int row = tid & 127, row_token = row / group;
+    const int row = tid & 127, row_token = row / group, row_head = row - row_token * group;
+    uint4* stage = reinterpret_cast<uint4*>(s_stage + warp * 1024);  // 16 rows of four 16-byte words
     const unsigned lanes = tmem + (static_cast<unsigned>(warp & 3) << 21);  // this warp's 32 lanes
     const unsigned at_s = lanes + 128 * x + 64 * half, at_o = lanes + 256 + 128 * x;
     const int meet = 1 + 4 * x + (warp & 3);  // the barrier of the two warps that share 32 rows
@@ -1023,42 +1050,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         two_warps_meet(meet);  // the next tile writes there
         const bool store = row_token < (x ? t.here_b : t.here_a);
         const float inv = ok ? 1.f / l : __int_as_float(0x7fc00000);
-        uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(P.out) +
-                                              (static_cast<int64_t>(t.begin + query) * P.heads +
-                                               static_cast<int64_t>(t.kv_head) * group + row % group) * P.width);
+        // A thread's row would leave by 16 bytes to each of 32 places at a time: 16 rows at a time go through
+        // shared memory instead and leave by four neighbouring words of eight rows.
+        uint16_t* out = static_cast<uint16_t*>(P.out) + (static_cast<int64_t>(t.begin + query) * P.heads +
+                                                         static_cast<int64_t>(t.kv_head) * group + row_head) * P.width;
+        const unsigned stores = __ballot_sync(kFull, store);
 #pragma unroll 1
         for (int i = 32 * half; i < DP; i += 64) {
           unsigned o[32];
-          __syncwarp();
           tc_load32(at_o + i, o);
           tc_wait_loads();
-          if (store && s_bad[tiles & 1]) {  // seen values that are not finite, taken out of the product above
-            for (int j = t.masked_from * kTcKeys; j <= query; ++j) {
-              const uint16_t* v = static_cast<const uint16_t*>(P.v) + (t.begin + j) * P.v_token + t.kv_head * P.v_head + i;
+          uint4 w[4];
 #pragma unroll
-              for (int u = 0; u < 32; ++u) {
-                if (i + u < P.width) {
-                  const float f = DT == COW_BF16 ? __uint_as_float(static_cast<unsigned>(v[u]) << 16)
-                                                 : __half2float(*reinterpret_cast<const __half*>(v + u));
-                  if (!(fabsf(f) < INFINITY)) o[u] = __float_as_uint(__uint_as_float(o[u]) + f);
-                }
-              }
-            }
+          for (int u = 0; u < 4; ++u) {
+            const unsigned* r = o + 8 * u;
+            w[u].x = pack2<DT>(__uint_as_float(r[0]) * inv, __uint_as_float(r[1]) * inv);
+            w[u].y = pack2<DT>(__uint_as_float(r[2]) * inv, __uint_as_float(r[3]) * inv);
+            w[u].z = pack2<DT>(__uint_as_float(r[4]) * inv, __uint_as_float(r[5]) * inv);
+            w[u].w = pack2<DT>(__uint_as_float(r[6]) * inv, __uint_as_float(r[7]) * inv);
           }
-          if (store) {
 #pragma unroll
-            for (int u = 0; u < 32; u += 8) {
-              if (i + u < P.width) {
-                uint4 w;
-                w.x = pack2<DT>(__uint_as_float(o[u]) * inv, __uint_as_float(o[u + 1]) * inv);
-                w.y = pack2<DT>(__uint_as_float(o[u + 2]) * inv, __uint_as_float(o[u + 3]) * inv);
-                w.z = pack2<DT>(__uint_as_float(o[u + 4]) * inv, __uint_as_float(o[u + 5]) * inv);
-                w.w = pack2<DT>(__uint_as_float(o[u + 6]) * inv, __uint_as_float(o[u + 7]) * inv);
-                out[(i + u) / 8] = w;
-              }
+          for (int part = 0; part < 2; ++part) {
+            if (lane / 16 == part) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) stage[lane % 16 * 4 + (u ^ (lane / 2 & 3))] = w[u];
             }
+            __syncwarp();
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int r = 8 * y + lane / 4, u = lane % 4, from = 16 * part + r;
+              uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(out), from));
+              if ((stores >> from & 1) && i + 8 * u < P.width)
+                *reinterpret_cast<uint4*>(to + i + 8 * u) = stage[4 * r + (u ^ (r / 2 & 3))];
+            }
+            __syncwarp();
           }
         }
+        if (store && s_bad[tiles & 1])
+          add_nonfinite<DT>(P, t.begin + t.masked_from * kTcKeys, t.begin + query, t.kv_head, out, 32 * half);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.o_empty[x]);
