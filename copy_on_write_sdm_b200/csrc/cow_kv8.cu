@@ -911,13 +911,6 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
       const float follow = step < -126 ? 0.f : pow2(step);
       a0 *= follow;
       a1 *= follow;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        o[i][0] *= a0;
-        o[i][1] *= a1;
-        o[i][2] *= a0;
-        o[i][3] *= a1;
-      }
       unsigned pa[4][2], pb[kSplit ? 4 : 1][2];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -950,12 +943,19 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
             zw[t] &= mask;
           }
         }
+        // The page's sum apart, then added in f32: the matrix unit's own adds do not round to nearest, and
+        // over thousands of pages that would show.
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const unsigned v0 = lo2(aw[t]), v1 = lo2(zw[t]), v2 = hi2(aw[t]), v3 = hi2(zw[t]);
-          mma_f16(o[i], v0, v1, v2, v3, pa[t][0], pa[t][1]);
-          if constexpr (kSplit) mma_f16(o[i], v0, v1, v2, v3, pb[t][0], pb[t][1]);
+          if constexpr (kSplit) mma_f16(y, v0, v1, v2, v3, pb[t][0], pb[t][1]);
+          mma_f16(y, v0, v1, v2, v3, pa[t][0], pa[t][1]);
         }
+        o[i][0] = fmaf(o[i][0], a0, y[0]);
+        o[i][1] = fmaf(o[i][1], a1, y[1]);
+        o[i][2] = fmaf(o[i][2], a0, y[2]);
+        o[i][3] = fmaf(o[i][3], a1, y[3]);
       }
       if (more) {
         copy(1, next_tile);

@@ -172,7 +172,7 @@ __device__ __forceinline__ void load_matrices_turned(unsigned* r, const __half* 
 }
 
 template <int D>
-__global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : 3) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
+__global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2 : 3) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
   using S = F32Shape<D>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __half* s_q = reinterpret_cast<__half*>(smem_raw);       // [2][kRows][kStride] hi, lo
@@ -360,17 +360,10 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : 3) cow_pro
     const float follow = step < -126 ? 0.f : pow2(step);
     a0 *= follow;
     a1 *= follow;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      o[i][0] *= a0;
-      o[i][1] *= a0;
-      o[i][2] *= a1;
-      o[i][3] *= a1;
-    }
     constexpr float kUp = 16384.f;
+    unsigned ph[4][4], pl[4][4];  // by 16 keys
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {  // 16 keys
-      unsigned ph[4], pl[4];
+    for (int n = 0; n < 4; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float e0 = exp2_fast(s[2 * n + x][0] - b0), e1 = exp2_fast(s[2 * n + x][1] - b0);
@@ -378,14 +371,20 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : 3) cow_pro
         l0 += e0 + e1;
         l1 += e2 + e3;
         const uint2 u = split2(e0 * shrink * kUp, e1 * shrink * kUp), w = split2(e2 * shrink * kUp, e3 * shrink * kUp);
-        ph[2 * x] = u.x;
-        ph[2 * x + 1] = w.x;
-        pl[2 * x] = u.y;
-        pl[2 * x + 1] = w.y;
+        ph[n][2 * x] = u.x;
+        ph[n][2 * x + 1] = w.x;
+        pl[n][2 * x] = u.y;
+        pl[n][2 * x + 1] = w.y;
       }
+    }
 #pragma unroll
-      for (int d = 0; d < D; d += 32) {
-        if (d >= W) break;
+    for (int d = 0; d < D; d += 32) {
+      if (d >= W) break;
+      // The tile's sum apart, then added in f32: the matrix unit's own adds do not round to nearest, and over
+      // a long prompt that would show.
+      float y[4][4] = {};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
         unsigned vh[8], vl[8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -394,11 +393,19 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : 3) cow_pro
           load_matrices_turned(vl + 4 * x, b + kKeys * S::kStride);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], pl, vh[2 * x], vh[2 * x + 1]);
+        for (int x = 0; x < 4; ++x) mma_f16(y[x], pl[n], vh[2 * x], vh[2 * x + 1]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], ph, vl[2 * x], vl[2 * x + 1]);
+        for (int x = 0; x < 4; ++x) mma_f16(y[x], ph[n], vl[2 * x], vl[2 * x + 1]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(o[d / 8 + x], ph, vh[2 * x], vh[2 * x + 1]);
+        for (int x = 0; x < 4; ++x) mma_f16(y[x], ph[n], vh[2 * x], vh[2 * x + 1]);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float* to = o[d / 8 + x];
+        to[0] = fmaf(to[0], a0, y[x][0]);
+        to[1] = fmaf(to[1], a0, y[x][1]);
+        to[2] = fmaf(to[2], a1, y[x][2]);
+        to[3] = fmaf(to[3], a1, y[x][3]);
       }
     }
   }
