@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kStoreThreads, DT == COW_F32 ? 3 : 5) cow_kv8_
 // another.  Values: the entries' slots fall into columns, aligned groups of four tokens of a page; a thread
 // reads a column's word at four neighbouring widths, turns the 4 x 4 codes about, and they leave
 // through shared memory as rows.
-// Bound: memory, (1 + element size) bytes for each element.
+// Bound: memory, (1 + element size) bytes for each element.  66,000 tokens of 8 heads of 128 to bf16: 86 us (4.7 TB/s).
 
 struct ReadLaunch {
   const uint8_t* codes[2];
@@ -386,6 +386,9 @@ __global__ void __launch_bounds__(kReadThreads) cow_kv8_read_kernel(const __grid
 //   held as two f16 parts (22 bits), and so are their probabilities.
 // * running maximum, sum and output of the softmax stay in f32 registers; value scales,
 //   powers of two, ride on the factor that rescales the output when the maximum moves.
+// Measured (32/8 heads of 128, bf16): 64 requests of 64 to 4,096 tokens 64 us (4.4 TB/s: 54 us of it the first kernel),
+// 4 of 65,536 102 us (5.3 TB/s, the first kernel 5.9); 16 of 256 to 512 tokens, 4 heads of 32, f32: 9.8 us, where
+// latency is all: 1.7 us until the lengths are scanned, 3.5 us for two pages, 1 us for the warps to meet.
 
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = 32 * kAttendWarps;
