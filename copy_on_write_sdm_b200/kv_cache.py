@@ -39,10 +39,16 @@ _STATUS_TEXT = [
 ]
 
 
+_ENTRIES: dict[str, object] = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(device: torch.device, what: str, *args) -> None:
     """One entry point on the device's current stream, the device made current where it is not."""
-    fn = getattr(_lib.load(), what)
-    if device.index == torch.cuda.current_device():
+    fn = _ENTRIES.get(what)
+    if fn is None:
+        fn = _ENTRIES[what] = getattr(_lib.load(), what)
+    if device.index == _current_device():
         rc = fn(*args, _lib.stream_of(device))
     else:
         with torch.cuda.device(device):
@@ -110,7 +116,7 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
         raise ValueError("queries, keys, values and starts must be on one device")
     if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
-    out = q.new_empty((tokens, heads, width))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _call(device, "cow_prompt_attention", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
           code, width ** -0.5 if scale is None else float(scale), out.data_ptr(), prompt_attention_status(device).data_ptr())
     return out
@@ -280,8 +286,7 @@ class PagedKVCache:
         if not 0 <= layer < self.layers:
             raise ValueError("the K/V cache has no such layer")
         code = _lib.dtype_code(dtype)
-        shape = (slots.shape[0], self.kv_heads, self.head_width)
-        keys, values = slots.new_empty(shape, dtype=dtype), slots.new_empty(shape, dtype=dtype)
+        keys, values = slots.new_empty((2, slots.shape[0], self.kv_heads, self.head_width), dtype=dtype).unbind()
         _call(self.device, "cow_kv8_read", self._at, layer, slots.data_ptr(), slots.shape[0], keys.data_ptr(),
               values.data_ptr(), code)
         return keys, values
@@ -308,7 +313,7 @@ class PagedKVCache:
             workspace = self._workspaces.get(heads)
             if workspace is None:
                 workspace = self._workspaces[heads] = self.new_workspace(heads)
-        out = q.new_empty(queries.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _call(self.device, "cow_kv8_attend", self._at, layer, q.data_ptr(), q0, q1, code, heads,
               self.head_width ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),
               workspace.numel())
