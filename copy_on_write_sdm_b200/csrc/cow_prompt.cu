@@ -50,6 +50,7 @@ struct Tile {
 // counts of kHeld sequences; those beyond 32 * kHeld are read again at every look.
 struct TileFinder {
   static constexpr int kHeld = 4;
+  int2 seq[kHeld];
   int held[kHeld];
   int most, all;
 
@@ -68,8 +69,10 @@ struct TileFinder {
     const int lane = threadIdx.x & 31;
     most = 0;
 #pragma unroll
+    for (int i = 0; i < kHeld; ++i) seq[i] = 32 * i + lane < P.sequences ? sequence_of(P, 32 * i + lane) : make_int2(0, 0);
+#pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-      held[i] = tiles_of(P, tile_tokens, 32 * i + lane);
+      held[i] = (seq[i].y + tile_tokens - 1) / tile_tokens;
       most = max(most, held[i]);
     }
     for (int b = 32 * kHeld + lane; b < P.sequences; b += 32) most = max(most, tiles_of(P, tile_tokens, b));
@@ -87,23 +90,26 @@ struct TileFinder {
       if (above(P, tile_tokens, mid) > x) lo = mid; else hi = mid;
     }
     int rank = x - above(P, tile_tokens, hi);  // among the sequences with more than lo tiles
-    int b = -1;
+    t.first = lo * tile_tokens;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
       const unsigned has = __ballot_sync(kFull, held[i] > lo);
-      if (b < 0 && rank < __popc(has)) b = 32 * i + nth_lane(has, rank);
+      if (rank >= 0 && rank < __popc(has)) {
+        const int from = nth_lane(has, rank);
+        t.begin = __shfl_sync(kFull, seq[i].x, from);
+        t.count = __shfl_sync(kFull, seq[i].y, from);
+      }
       rank -= __popc(has);
     }
-    for (int base = 32 * kHeld; b < 0 && base < P.sequences; base += 32) {
+    for (int base = 32 * kHeld; rank >= 0 && base < P.sequences; base += 32) {
       const unsigned has = __ballot_sync(kFull, tiles_of(P, tile_tokens, base + lane) > lo);
-      if (rank < __popc(has)) b = base + nth_lane(has, rank);
+      if (rank < __popc(has)) {
+        const int2 found = sequence_of(P, base + nth_lane(has, rank));
+        t.begin = found.x;
+        t.count = found.y;
+      }
       rank -= __popc(has);
     }
-    if (b < 0) return t;
-    const int2 seq = sequence_of(P, b);
-    t.begin = seq.x;
-    t.count = seq.y;
-    t.first = lo * tile_tokens;
     return t;
   }
 };
@@ -126,8 +132,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 2^14 down; value scales ride on the factor that rescales the output when a maximum moves.
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
-// Measured: sixteen prompts of 256, four heads of 32: 14.5 us a call (31 us with the f32 pipe); 16 x 1,024 tokens,
-// 32/8 heads of 128: 2.0 ms, 67 TFLOP/s of f32 work (200 of f16 products).  Bound: latency at the small
+// Measured: sixteen prompts of 256, four heads of 32: 14.4 us a call (31 us with the f32 pipe); 16 x 1,024 tokens,
+// 32/8 heads of 128: 1.69 ms, 82 TFLOP/s of f32 work (245 of f16 products).  Bound: latency at the small
 // size, at the large one reading the split tiles out of shared memory beside the matrix instructions.
 
 constexpr int kKeys = 64;
@@ -172,6 +178,18 @@ __device__ __forceinline__ void load_matrices_turned(unsigned* r, const __half* 
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_addr(at))
                : "memory");
+}
+
+// Adds to a row's output the values of tokens 0..last that are not finite, at two of every eight widths from `from` on.
+__device__ __noinline__ void add_nonfinite_f32(const float* v, int64_t v_token, int last, float* out, int from, int width) {
+  for (int d = from; d < width; d += d % 2 ? 7 : 1) {
+    float sum = out[d];
+    for (int j = 0; j <= last; ++j) {
+      const float x = v[j * v_token + d];
+      if (!(fabsf(x) < INFINITY)) sum += x;
+    }
+    out[d] = sum;
+  }
 }
 
 template <int D>
@@ -429,16 +447,9 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     for (int i = 0; i < D / 8; ++i) {
       const int d = 8 * i + 2 * c;
       if (d >= W) continue;
-      float2 y = make_float2(o[i][2 * half] * down * inv, o[i][2 * half + 1] * down * inv);
-      if (s_bad) {  // seen values that are not finite
-        for (int j = 0; j <= query; ++j) {
-          const float2 x = __ldg(reinterpret_cast<const float2*>(V + (t.begin + j) * P.v_token + d));
-          if (!(fabsf(x.x) < INFINITY)) y.x += x.x;
-          if (!(fabsf(x.y) < INFINITY)) y.y += x.y;
-        }
-      }
-      *reinterpret_cast<float2*>(out + d) = y;
+      *reinterpret_cast<float2*>(out + d) = make_float2(o[i][2 * half] * down * inv, o[i][2 * half + 1] * down * inv);
     }
+    if (s_bad) add_nonfinite_f32(V + t.begin * P.v_token, P.v_token, query, out, 2 * c, W);
   }
 }
 
@@ -598,13 +609,6 @@ __device__ __forceinline__ void tc_load32(unsigned at, unsigned* r) {
       "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : COW_R8(r, 0), COW_R8(r, 8), COW_R8(r, 16), COW_R8(r, 24)
       : "r"(at));
-}
-__device__ __forceinline__ void tc_store32(unsigned at, const unsigned* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::COW_W8(r, 0),
-      COW_W8(r, 8), COW_W8(r, 16), COW_W8(r, 24), "r"(at)
-      : "memory");
 }
 __device__ __forceinline__ void tc_load8(unsigned at, unsigned* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : COW_R8(r, 0) : "r"(at));
