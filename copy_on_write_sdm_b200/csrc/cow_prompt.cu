@@ -133,7 +133,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
 // Measured: sixteen prompts of 256, four heads of 32: 14.4 us a call (31 us with the f32 pipe); 16 x 1,024 tokens,
-// 32/8 heads of 128: 1.69 ms, 82 TFLOP/s of f32 work (245 of f16 products).  Bound: latency at the small
+// 32/8 heads of 128: 1.55 ms, 89 TFLOP/s of f32 work (266 of f16 products).  Bound: latency at the small
 // size, at the large one reading the split tiles out of shared memory beside the matrix instructions.
 
 constexpr int kKeys = 64;
@@ -156,11 +156,44 @@ __device__ __forceinline__ unsigned pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const unsigned*>(&h);
 }
-// hi and lo parts of a and b; lo is 0 where hi is not finite
-__device__ __forceinline__ uint2 split2(float a, float b) {
-  const unsigned hi = pack_half2(a, b);
+// pairs of floats in one 64-bit register
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t r) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// hi and lo parts of a and b, whose magnitudes are below 2^16; lo of what is not finite is NaN
+__device__ __forceinline__ uint2 split2(uint64_t x) {
+  const float2 f = both(x);
+  const unsigned hi = pack_half2(f.x, f.y);
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return make_uint2(hi, pack_half2(fabsf(h.x) < INFINITY ? a - h.x : 0.f, fabsf(h.y) < INFINITY ? b - h.y : 0.f));
+  const float2 l = both(fma2(pair(h.x, h.y), pair(-1.f, -1.f), x));
+  return make_uint2(hi, pack_half2(l.x, l.y));
 }
 __device__ __forceinline__ void mma_f16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -260,11 +293,17 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 #pragma unroll
       for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
       const int scale = split_exponent(most);
-      const float up = pow2(scale);
+      const float up = P.scale_log2 < 0.f ? -pow2(scale) : pow2(scale);
       if (d == 0) s_row[r] = scale;
-      const uint2 a = split2(x[i].x * up, x[i].y * up), b = split2(x[i].z * up, x[i].w * up);
-      *reinterpret_cast<uint2*>(s_q + r * S::kStride + d) = make_uint2(a.x, b.x);
-      *reinterpret_cast<uint2*>(s_q + (S::kRows + r) * S::kStride + d) = make_uint2(a.y, b.y);
+      const uint2 a = split2(pair(e[0] * up, e[1] * up)), b = split2(pair(e[2] * up, e[3] * up));
+      __half* to = s_q + r * S::kStride + d;
+      *reinterpret_cast<uint2*>(to) = make_uint2(a.x, b.x);
+      *reinterpret_cast<uint2*>(to + S::kRows * S::kStride) = make_uint2(a.y, b.y);
+      if (!(fabsf(e[0] + e[1] + e[2] + e[3]) < INFINITY)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (!(fabsf(e[u]) < INFINITY)) to[S::kRows * S::kStride + u] = __float2half(0.f);
+      }
     }
   }
   load(0);
@@ -277,42 +316,58 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   int unit = 0;  // the output is held times 2^(unit + 14)
+  const float scale = fabsf(P.scale_log2);
 
   for (int j0 = 0; j0 < last; j0 += kKeys) {
     // the tile's scales, over the block
     float mk = 0.f, mv = 0.f;
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
-      const float a[4] = {k[i].x, k[i].y, k[i].z, k[i].w}, b[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      mk = max3_nan(max3_nan(mk, fabsf(k[i].x), fabsf(k[i].y)), fabsf(k[i].z), fabsf(k[i].w));
+      mv = max3_nan(max3_nan(mv, fabsf(v[i].x), fabsf(v[i].y)), fabsf(v[i].z), fabsf(v[i].w));
+    }
+    const bool odd_k = !(mk < INFINITY), odd_v = !(mv < INFINITY);
+    if (odd_k || odd_v) {  // seldom: the largest of the finite ones, and values that are not finite are left out
+      auto most_of = [](float most, float x) { return fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most; };
+      auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
+      mk = mv = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (fabsf(a[u]) < INFINITY) mk = fmaxf(mk, fabsf(a[u]));
-        if (fabsf(b[u]) < INFINITY) mv = fmaxf(mv, fabsf(b[u]));
-        else bad = true;
+      for (int i = 0; i < S::kVecs; ++i) {
+        mk = most_of(most_of(most_of(most_of(mk, k[i].x), k[i].y), k[i].z), k[i].w);
+        mv = most_of(most_of(most_of(most_of(mv, v[i].x), v[i].y), v[i].z), v[i].w);
+        v[i] = make_float4(finite(v[i].x), finite(v[i].y), finite(v[i].z), finite(v[i].w));
       }
+      if (odd_v) s_bad = 1;
     }
     const int2 found = make_int2(__reduce_max_sync(kFull, __float_as_int(mk)), __reduce_max_sync(kFull, __float_as_int(mv)));
     if (lane == 0) s_most[warp] = found;
-    if (bad) s_bad = 1;
     __syncthreads();  // also: the last tile is used up
     int2 most = s_most[0];
 #pragma unroll
     for (int w = 1; w < S::kWarps; ++w) most = make_int2(max(most.x, s_most[w].x), max(most.y, s_most[w].y));
     const int ek = split_exponent(__int_as_float(most.x));
     const int ev = most.y > 0 ? split_exponent(__int_as_float(most.y)) : unit;
-    const float uk = pow2(ek), uv = pow2(ev);
+    const uint64_t uk = pair(pow2(ek), pow2(ek)), uv = pair(pow2(ev), pow2(ev));
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
       const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
-      uint2 a = split2(k[i].x * uk, k[i].y * uk), b = split2(k[i].z * uk, k[i].w * uk);
+      uint2 a = split2(mul2(pair(k[i].x, k[i].y), uk)), b = split2(mul2(pair(k[i].z, k[i].w), uk));
       *reinterpret_cast<uint2*>(s_k + at) = make_uint2(a.x, b.x);
       *reinterpret_cast<uint2*>(s_k + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
-      auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
-      a = split2(finite(v[i].x) * uv, finite(v[i].y) * uv);
-      b = split2(finite(v[i].z) * uv, finite(v[i].w) * uv);
+      a = split2(mul2(pair(v[i].x, v[i].y), uv));
+      b = split2(mul2(pair(v[i].z, v[i].w), uv));
       *reinterpret_cast<uint2*>(s_v + at) = make_uint2(a.x, b.x);
       *reinterpret_cast<uint2*>(s_v + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
+    }
+    if (odd_k) {  // a key that is not finite has no lo part, so that its score is infinite and not NaN
+#pragma unroll
+      for (int i = 0; i < S::kVecs; ++i) {
+        const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
+        const float e[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (!(fabsf(e[u]) < INFINITY)) s_k[kKeys * S::kStride + at + u] = __float2half(0.f);
+      }
     }
     __syncthreads();
     if (j0 + kKeys < last) load(j0 + kKeys);
@@ -344,15 +399,23 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       }
     }
     // softmax: columns 8 n + 2 c and the next of rows row0, row0 + 8
-    const float f0 = pow2(min(max(-sq0 - ek, -126), 127)) * P.scale_log2, f1 = pow2(min(max(-sq1 - ek, -126), 127)) * P.scale_log2;
+    constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
+    // factors of the scores, above 0 so that a masked one stays -inf (the scale's sign is in the queries)
+    const float f0 = fmaxf(pow2(min(max(-sq0 - ek, -126), 127)) * scale, kLeast);
+    const float f1 = fmaxf(pow2(min(max(-sq1 - ek, -126), 127)) * scale, kLeast);
+    if (j0 + kKeys - 1 > t.first) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int key = j0 + 8 * n + 2 * c;
+        if (key > query0) s[n][0] = -INFINITY;
+        if (key + 1 > query0) s[n][1] = -INFINITY;
+        if (key > query1) s[n][2] = -INFINITY;
+        if (key + 1 > query1) s[n][3] = -INFINITY;
+      }
+    }
     float big0 = -INFINITY, big1 = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const int key = j0 + 8 * n + 2 * c;
-      s[n][0] = key <= query0 ? s[n][0] * f0 : -INFINITY;
-      s[n][1] = key + 1 <= query0 ? s[n][1] * f0 : -INFINITY;
-      s[n][2] = key <= query1 ? s[n][2] * f1 : -INFINITY;
-      s[n][3] = key + 1 <= query1 ? s[n][3] * f1 : -INFINITY;
       big0 = fmaxf(big0, fmaxf(s[n][0], s[n][1]));
       big1 = fmaxf(big1, fmaxf(s[n][2], s[n][3]));
     }
@@ -361,7 +424,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, x));
       big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, x));
     }
-    const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
+    const float n0 = fmaxf(m0, big0 * f0), n1 = fmaxf(m1, big1 * f1);
     const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;  // all -inf so far: weights 0
     float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
     m0 = n0;
@@ -381,22 +444,27 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     const float follow = step < -126 ? 0.f : pow2(step);
     a0 *= follow;
     a1 *= follow;
-    constexpr float kUp = 16384.f;
+    const uint64_t f00 = pair(f0, f0), f11 = pair(f1, f1), b00 = pair(-b0, -b0), b11 = pair(-b1, -b1);
+    uint64_t e0[8], e1[8], sum0 = pair(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 y0 = both(fma2(pair(s[n][0], s[n][1]), f00, b00)), y1 = both(fma2(pair(s[n][2], s[n][3]), f11, b11));
+      e0[n] = pair(exp2_fast(y0.x), exp2_fast(y0.y));
+      e1[n] = pair(exp2_fast(y1.x), exp2_fast(y1.y));
+      sum0 = add2(sum0, e0[n]);
+      sum1 = add2(sum1, e1[n]);
+    }
+    l0 += both(sum0).x + both(sum0).y;
+    l1 += both(sum1).x + both(sum1).y;
+    const uint64_t up = pair(shrink * 16384.f, shrink * 16384.f);
     unsigned ph[4][4], pl[4][4];  // by 16 keys
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float e0 = exp2_fast(s[2 * n + x][0] - b0), e1 = exp2_fast(s[2 * n + x][1] - b0);
-        const float e2 = exp2_fast(s[2 * n + x][2] - b1), e3 = exp2_fast(s[2 * n + x][3] - b1);
-        l0 += e0 + e1;
-        l1 += e2 + e3;
-        const uint2 u = split2(e0 * shrink * kUp, e1 * shrink * kUp), w = split2(e2 * shrink * kUp, e3 * shrink * kUp);
-        ph[n][2 * x] = u.x;
-        ph[n][2 * x + 1] = w.x;
-        pl[n][2 * x] = u.y;
-        pl[n][2 * x + 1] = w.y;
-      }
+    for (int n = 0; n < 8; ++n) {
+      const uint2 u = split2(mul2(e0[n], up)), w = split2(mul2(e1[n], up));
+      ph[n / 2][2 * (n % 2)] = u.x;
+      ph[n / 2][2 * (n % 2) + 1] = w.x;
+      pl[n / 2][2 * (n % 2)] = u.y;
+      pl[n / 2][2 * (n % 2) + 1] = w.y;
     }
 #pragma unroll
     for (int d = 0; d < D; d += 32) {
@@ -644,33 +712,6 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
     return *reinterpret_cast<const unsigned*>(&h);
   }
 }
-// pairs of floats in one 64-bit register
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 both(uint64_t r) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // 2^y of both halves on the multiply-add pipe, for y <= about 100: with n the nearest integer, f = y - n in
 // [-1/2, 1/2] and 2^f a polynomial with constant term 1, fitted here by reweighted least squares to
 // the relative error (degree 3: 1.0e-4, degree 4: 2.8e-6, below the rounding of a weight to bf16, f16).
