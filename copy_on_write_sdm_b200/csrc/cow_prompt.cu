@@ -132,8 +132,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 2^14 down; value scales ride on the factor that rescales the output when a maximum moves.
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
-// Measured: sixteen prompts of 256, four heads of 32: 14.4 us a call (31 us with the f32 pipe); 16 x 1,024 tokens,
-// 32/8 heads of 128: 1.55 ms, 89 TFLOP/s of f32 work (266 of f16 products).  Bound: latency at the small
+// Measured: sixteen prompts of 256, four heads of 32: 14.0 us back to back (31 us with the f32 pipe); 16 x 1,024 tokens,
+// 32/8 heads of 128: 1.54 ms, 89 TFLOP/s of f32 work (266 of f16 products).  Bound: latency at the small
 // size, at the large one reading the split tiles out of shared memory beside the matrix instructions.
 
 constexpr int kKeys = 64;
@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       }
     }
   };
+  load(0);
   // queries: a warp's own 16 rows, kLanes lanes to a row, all loads under way before the first is used
   {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kTurns = 16 / kAtOnce;
@@ -306,7 +307,6 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       }
     }
   }
-  load(0);
   __syncwarp();
   const int row0 = 16 * warp + g;  // this lane's rows: row0 and row0 + 8
   const int query0 = t.first + row0 / group, query1 = t.first + (row0 + 8) / group;  // their places in the sequence
