@@ -613,6 +613,9 @@ __device__ __forceinline__ bool any_of_two_warps(int id, bool yes) {
 }
 __device__ __forceinline__ void two_warps_meet(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ unsigned long long nanoseconds() {
   unsigned long long t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
@@ -678,6 +681,17 @@ __device__ __forceinline__ void tc_load32(unsigned at, unsigned* r) {
       : COW_R8(r, 0), COW_R8(r, 8), COW_R8(r, 16), COW_R8(r, 24)
       : "r"(at));
 }
+// 16 columns, complete after tc_wait_loads16 of the same registers
+__device__ __forceinline__ void tc_load16(unsigned at, unsigned* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : COW_R8(r, 0), COW_R8(r, 8)
+               : "r"(at));
+}
+#define COW_RW8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+__device__ __forceinline__ void tc_wait_loads16(unsigned* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : COW_RW8(r, 0), COW_RW8(r, 8)::"memory");
+}
+#undef COW_RW8
 __device__ __forceinline__ void tc_load8(unsigned at, unsigned* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : COW_R8(r, 0) : "r"(at));
 }
@@ -747,14 +761,14 @@ __device__ __forceinline__ unsigned zero_times(unsigned w, unsigned sum) {
   return r;
 }
 
-// Adds to a row's output the values of tokens first..last that are not finite: those of every 32 columns of
+// Adds to a row's output the values of tokens first..last that are not finite: those of every 16 columns of
 // two, from column `from` on.
 template <int DT>
 __device__ __noinline__ void add_nonfinite(const PromptLaunch& P, int first, int last, int kv_head, uint16_t* out, int from) {
   auto value = [](uint16_t u) {
     return DT == COW_BF16 ? __uint_as_float(static_cast<unsigned>(u) << 16) : __half2float(*reinterpret_cast<const __half*>(&u));
   };
-  for (int d = from; d < P.width; d += d % 32 == 31 ? 33 : 1) {
+  for (int d = from; d < P.width; d += d % 16 == 15 ? 17 : 1) {
     float sum = value(out[d]);
     for (int j = first; j <= last; ++j) {
       const float f = value(static_cast<const uint16_t*>(P.v)[j * P.v_token + kv_head * P.v_head + d]);
@@ -783,6 +797,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   uint8_t* s_stage = s_ring + S::kSlots * S::kTileBytes;
 
   if (warp == 16) {
+    if (elect_one()) {
+      prefetch_map(&L.q);
+      prefetch_map(&L.k);
+      prefetch_map(&L.v);
+    }
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (warp == 17 && lane == 0) {
@@ -987,13 +1007,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         ++looks[k];
         uint4* words = reinterpret_cast<uint4*>(s_ring + (i % S::kSlots) * S::kTileBytes);
         constexpr int kEach = S::kTileBytes / 16 / 32;
-        unsigned sum = 0;  // of 0 times each value, by halves: NaN once one is not finite
+        unsigned sum[4] = {};  // of 0 times each value, by halves: NaN once one is not finite; four, as each waits for its last
 #pragma unroll 8
         for (int u = 0; u < kEach; ++u) {
           const uint4 w = words[u * 32 + lane];
-          sum = zero_times<DT>(w.x, zero_times<DT>(w.y, zero_times<DT>(w.z, zero_times<DT>(w.w, sum))));
+          sum[0] = zero_times<DT>(w.x, sum[0]);
+          sum[1] = zero_times<DT>(w.y, sum[1]);
+          sum[2] = zero_times<DT>(w.z, sum[2]);
+          sum[3] = zero_times<DT>(w.w, sum[3]);
         }
-        if ((sum & 0x7fff7fffu) != 0) {
+        if (((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0) {
           constexpr unsigned kExp = DT == COW_BF16 ? 0x7f80u : 0x7c00u;
           s_bad[tiles & 1] = 1;
           for (int u = 0; u < kEach; ++u) {
@@ -1015,16 +1038,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
     // ---- softmax
     const int x = warp >> 3, half = (warp >> 2) & 1;  // this thread's half of the keys
     const int row = tid & 127, row_token = row / group, row_head = row - row_token * group;
-    uint4* stage = reinterpret_cast<uint4*>(s_stage + warp * 1024);  // 16 rows of four 16-byte words
+    uint4* stage = reinterpret_cast<uint4*>(s_stage + warp * 1024);  // 32 rows of two 16-byte words
     const unsigned lanes = tmem + (static_cast<unsigned>(warp & 3) << 21);  // this warp's 32 lanes
     const unsigned at_s = lanes + 128 * x + 64 * half, at_o = lanes + 256 + 128 * x;
     const int meet = 1 + 4 * x + (warp & 3);  // the barrier of the two warps that share 32 rows
     const float c = fabsf(P.scale_log2);
     unsigned steps = 0, done = 0;
     bool ok = true;
-    for (int tiles = 0; ok; ++tiles) {
+    for (int tiles = 0;; ++tiles) {
       // A wait that gave up is only remembered: both warps of a pair go on to their common end of the tile.
-      if (any_of_two_warps(meet, !wait(&bars.tile_full[tiles & 1], (tiles >> 1) & 1))) break;
+      if (any_of_two_warps(meet, !ok || !wait(&bars.tile_full[tiles & 1], (tiles >> 1) & 1))) break;
       const TcTile& t = s_tiles[tiles & 1];
       if (t.count == 0) break;
       const int nx = x ? t.n_b : t.n_a;
@@ -1106,56 +1129,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
         l += sums.x + sums.y;
       }
       if (nx > 0) {
-        ok = wait(&bars.o_full[x], done & 1) && ok;
-        ++done;
-        tc_fence_after();
-        s_most[x][half][row] = l;
-        ok = !any_of_two_warps(meet, !ok);
+        // The sums meet while the last products run; of a wait that gave up they make NaN.
+        s_most[x][half][row] = ok ? l : __int_as_float(0x7fc00000);
+        two_warps_meet(meet);
         l += s_most[x][half ^ 1][row];
-        two_warps_meet(meet);  // the next tile writes there
         const bool store = row_token < (x ? t.here_b : t.here_a);
-        const float inv = ok ? 1.f / l : __int_as_float(0x7fc00000);
-        // A thread's row would leave by 16 bytes to each of 32 places at a time: 16 rows at a time go through
-        // shared memory instead and leave by four neighbouring words of eight rows.
+        const float whole = 1.f / l;
         uint16_t* out = static_cast<uint16_t*>(P.out) + (static_cast<int64_t>(t.begin + query) * P.heads +
                                                          static_cast<int64_t>(t.kv_head) * group + row_head) * P.width;
-        const unsigned stores = __ballot_sync(kFull, store);
+        // A thread's row would leave by 16 bytes to each of 32 places at a time: 16 columns of the warp's rows go
+        // through shared memory instead and leave by two neighbouring words of 16 rows.  This lane's places:
+        uint16_t* to[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          to[y] = reinterpret_cast<uint16_t*>(__shfl_sync(kFull, store ? reinterpret_cast<unsigned long long>(out) : 0ull, 16 * y + lane / 2));
+        const int at_w = 2 * lane, turn_w = lane >> 2 & 1, at_r = lane ^ (lane >> 3 & 1);
+        ok = __all_sync(kFull, wait(&bars.o_full[x], done & 1)) && ok;
+        ++done;
+        tc_fence_after();
+        const float inv = ok ? whole : __int_as_float(0x7fc00000);
+        const uint64_t inv2 = pair(inv, inv);
+        const bool bad = s_bad[tiles & 1];
 #pragma unroll 1
-        for (int i = 32 * half; i < DP; i += 64) {
-          unsigned o[32];
-          tc_load32(at_o + i, o);
-          tc_wait_loads();
-          uint4 w[4];
+        for (int n = 0; n < DP / 32; ++n) {
+          unsigned r[16];
+          tc_load16(at_o + 32 * n + 16 * half, r);
+          tc_wait_loads16(r);
+          unsigned w[8];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const unsigned* r = o + 8 * u;
-            w[u].x = pack2<DT>(__uint_as_float(r[0]) * inv, __uint_as_float(r[1]) * inv);
-            w[u].y = pack2<DT>(__uint_as_float(r[2]) * inv, __uint_as_float(r[3]) * inv);
-            w[u].z = pack2<DT>(__uint_as_float(r[4]) * inv, __uint_as_float(r[5]) * inv);
-            w[u].w = pack2<DT>(__uint_as_float(r[6]) * inv, __uint_as_float(r[7]) * inv);
+          for (int u = 0; u < 8; ++u) {
+            const float2 f = both(mul2(pair(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), inv2));
+            w[u] = pack2<DT>(f.x, f.y);
           }
+          stage[at_w + turn_w] = make_uint4(w[0], w[1], w[2], w[3]);
+          stage[at_w + (turn_w ^ 1)] = make_uint4(w[4], w[5], w[6], w[7]);
+          __syncwarp();
+          const int d = 32 * n + 16 * half + 8 * (lane & 1);
+          if (d < P.width) {
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            if (lane / 16 == part) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) stage[lane % 16 * 4 + (u ^ (lane / 2 & 3))] = w[u];
-            }
-            __syncwarp();
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const int r = 8 * y + lane / 4, u = lane % 4, from = 16 * part + r;
-              uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(out), from));
-              if ((stores >> from & 1) && i + 8 * u < P.width)
-                *reinterpret_cast<uint4*>(to + i + 8 * u) = stage[4 * r + (u ^ (r / 2 & 3))];
-            }
-            __syncwarp();
+            for (int y = 0; y < 2; ++y)
+              if (to[y]) *reinterpret_cast<uint4*>(to[y] + d) = stage[32 * y + at_r];
           }
+          __syncwarp();
         }
-        if (store && s_bad[tiles & 1])
-          add_nonfinite<DT>(P, t.begin + t.masked_from * kTcKeys, t.begin + query, t.kv_head, out, 32 * half);
         tc_fence_before();
-        __syncwarp();
         if (lane == 0) mbar_arrive(&bars.o_empty[x]);
+        if (bad && store)
+          add_nonfinite<DT>(P, t.begin + t.masked_from * kTcKeys, t.begin + query, t.kv_head, out, 16 * half);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.tile_empty[tiles & 1]);
