@@ -133,8 +133,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
 // Measured: sixteen prompts of 256, four heads of 32: 14.0 us back to back (31 us with the f32 pipe); 16 x 1,024 tokens,
-// 32/8 heads of 128: 1.54 ms, 89 TFLOP/s of f32 work (266 of f16 products).  Bound: latency at the small
-// size, at the large one reading the split tiles out of shared memory beside the matrix instructions.
+// 32/8 heads of 128: 1.54 ms, 89 TFLOP/s of f32 work (266 of f16 products, of about 560 that `mma.sync` gives here:
+// 1,024 multiply-adds a cycle and SM).  Bound: the chain of split, scores, softmax and products of a key
+// tile, with two or three warps to a scheduler: a third of the issue slots and half of the matrix rate are in use.  What
+// shortened it was fewer instructions (packed pairs, rare cases on paths of their own: 1.69 -> 1.55 ms).  Tried
+// and not kept: two split tiles in turn with the next split beside the products, eight sums in turn instead of
+// four (no change); tiles of 32 keys (1.72 ms), four warps twice an SM (2.0 ms), 128 keys for width 32.
 
 constexpr int kKeys = 64;
 
@@ -546,14 +550,17 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 // them have them added at the end.
 //
 // A block stays and takes tile after tile: loads and scores of the next begin under the end of the last.
-// Measured (bf16): 2 x 8,192 tokens, 32/8 heads of 128: 0.92-1.03 ms, 1,070-1,200 TFLOP/s back to back under the power
-// cap (a cuBLAS product sustains 1,384 there, 1,658 in a burst); 32 requests of 64 to 2,048, 16/4 heads of 64: 190 us,
-// 543 TFLOP/s.  Bound: the chain from a tile's scores through its softmax (1,750 cycles) and the two products
-// (768 after the first half of P) back to its next scores, 2,900 cycles for the 2,048 of tensor work of both tiles;
-// for narrow heads the 48 special-function and 370 other instructions of a warp for 32 rows of 64 keys; for short
-// prompts what a tile costs beside its key tiles, 4,000 cycles.  Tried and not kept: a thread for each row with all
-// 128 scores in registers (3,430 cycles a step), issue threads of A's and of B's own (they fall into step with
-// each other: 4,200), three score tiles in turn for widths to 64 (the softmax is the bound: no change).
+// Measured (bf16): 2 x 8,192 tokens, 32/8 heads of 128: 0.95-1.03 ms, 1,070-1,160 TFLOP/s back to back under the power
+// cap (a cuBLAS product sustains 1,384 there, 1,658 in a burst); 32 requests of 64 to 2,048, 16/4 heads of 64: 193 us,
+// 533 TFLOP/s; 21 of 1 to 777, 14/2 heads of 96 (f16): 35 us.  Bound: the chain from a tile's scores through its softmax
+// (1,750 cycles) and the two products (768 after the first half of P) back to its next scores, 2,900 cycles for the
+// 2,048 of tensor work of both tiles; for narrow heads the 48 special-function and 370 other instructions of a warp for
+// 32 rows of 64 keys; for short prompts what a tile costs beside its key tiles, 4,000 cycles (last products,
+// 1,200; output, 2,000; next tile and its scores, 1,500, partly under the other tile's softmax).  Tried and not kept:
+// a thread for each row with all 128 scores in registers (3,430 cycles a step), issue threads of A's and of B's own
+// (they fall into step with each other: 4,200), three score tiles in turn for widths to 64 (the softmax is the
+// bound: no change), the output given up as soon as it is in registers (the same: 1 % slower), masked tiles looked
+// through only where some row does not see them, and from a step earlier (no change).
 // Of eight pairs of weights, two come from the polynomial (0: 395,000 cycles for 8,192 tokens of
 // 16/4 heads of 64, 2: 354,000, 3: 369,000).
 // Every wait is bounded; one that gives up sets a status bit and ends the block, its current rows NaN.
