@@ -152,6 +152,7 @@ struct F32Shape {
   static constexpr int kBytes = 2 * (2 * kRows + 4 * kKeys) * kStride;
 };
 
+constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
 // The exponent of the scale that brings `most` (finite, >= 0) to [2^14, 2^15), as far as both are normal.
 __device__ __forceinline__ int split_exponent(float most) { return min(max(14 - ((__float_as_int(most) >> 23) - 127), -113), 100); }
@@ -363,14 +364,17 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       *reinterpret_cast<uint2*>(s_v + at) = make_uint2(a.x, b.x);
       *reinterpret_cast<uint2*>(s_v + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
     }
-    if (odd_k) {  // a key that is not finite has no lo part, so that its score is infinite and not NaN
+    if (odd_k) {  // what is not finite of a key meets hi parts of the queries alone: of a lo part 0 or of another sign it makes NaN
 #pragma unroll
       for (int i = 0; i < S::kVecs; ++i) {
         const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
         const float e[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (!(fabsf(e[u]) < INFINITY)) s_k[kKeys * S::kStride + at + u] = __float2half(0.f);
+          if (!(fabsf(e[u]) < INFINITY)) {
+            s_k[at + u] = __float2half(0.f);
+            s_k[kKeys * S::kStride + at + u] = __float2half(e[u]);
+          }
       }
     }
     __syncthreads();
@@ -403,7 +407,6 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       }
     }
     // softmax: columns 8 n + 2 c and the next of rows row0, row0 + 8
-    constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
     // factors of the scores, above 0 so that a masked one stays -inf (the scale's sign is in the queries)
     const float f0 = fmaxf(pow2(min(max(-sq0 - ek, -126), 127)) * scale, kLeast);
     const float f1 = fmaxf(pow2(min(max(-sq1 - ek, -126), 127)) * scale, kLeast);
@@ -1296,10 +1299,12 @@ int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_
       !rows_ok(keys, key_token_stride, key_head_stride, dtype) ||
       !rows_ok(values, value_token_stride, value_head_stride, dtype) || !starts || !out || !aligned16(out))
     return COW_ERR_INVALID;
+  // not 0, so that a masked score times it stays -inf
+  const float scale_log2 = scale * 1.4426950408889634f;
   PromptLaunch P{queries, keys, values, out, starts, query_token_stride, query_head_stride, key_token_stride,
                  key_head_stride, value_token_stride, value_head_stride, status, static_cast<int32_t>(sequences),
                  static_cast<int32_t>(tokens), heads, kv_heads, heads / kv_heads, width, dtype,
-                 scale * 1.4426950408889634f};
+                 fabsf(scale_log2) < kLeast ? kLeast : scale_log2};
   return dtype == COW_F32 ? prompt_f32(P, as_stream(stream)) : prompt_tc(P, as_stream(stream));
 }
 

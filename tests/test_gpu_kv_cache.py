@@ -265,6 +265,13 @@ def test_attend_matches_the_plain_form(dev, dtype, lengths, heads, group, width)
             assert_attention(got, want, q=_np(q), k=np.concatenate(k), v=np.concatenate(v), scale=s)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attend_with_a_scale_of_zero_weighs_all_tokens_alike(dev, dtype):
+    cache, k, v = _filled(dev, [70, 1, 200], 2, 64, dtype, 3)
+    q = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(4)).to(dev, dtype)
+    assert_attention(cache.attend(q, scale=0.0), O.attend(_np(q), k, v, 0.0), q=_np(q), k=np.concatenate(k), v=np.concatenate(v), scale=0.0)
+
+
 @pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
 def test_attend_over_long_and_short_requests_together(dev, dtype):
     """Runs of many blocks, joined; and runs of many requests in one block."""

@@ -106,6 +106,24 @@ def test_what_a_query_does_not_see_does_not_touch_it(dev, dtype, bad):  # noqa: 
             assert not torch.isfinite(got[at:237, :2]).any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_scale_of_zero_weighs_all_tokens_alike(dev, dtype):  # noqa: F811
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    q, k, v, starts, device_starts = _inputs(dev, [300, 17], 2, 2, 64, dtype, 5)
+    _check(prompt_attention(q, k, v, device_starts, scale=0.0), q, k, v, starts, 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_infinite_key_of_score_minus_infinity_has_no_weight(dev, dtype):  # noqa: F811
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    q, k, v, starts, device_starts = _inputs(dev, [200, 150], 2, 2, 64, dtype, 6)
+    q[..., 3] = -q[..., 3].abs() - 0.5
+    k[[20, 220], :, 3] = float("inf")
+    _check(prompt_attention(q, k, v, device_starts), q, k, v, starts)
+
+
 def test_tokens_outside_every_sequence(dev):  # noqa: F811
     from copy_on_write_sdm_b200 import prompt_attention
 
