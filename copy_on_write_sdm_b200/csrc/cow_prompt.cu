@@ -124,12 +124,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // f32
 // --------------------------------------------------------------------------
 //
-// Each operand is held as two f16 parts, hi and lo, after a scale by a power of two that brings its row's
-// (queries) or tile's (keys, values) largest magnitude to [2^14, 2^15): 22 bits of it, and three of the four
-// part products on the f16 matrix instructions with f32 sums, lo * lo being below the others' rounding.  That
-// is f32's accuracy to a few units at a third of the f16 rate, several times what the f32 pipe
-// gives.  A tile of 64 keys is split once for the whole block.  Probabilities are split the same way, from
-// 2^14 down; value scales ride on the factor that rescales the output when a maximum moves.
+// Queries and keys are held as three bf16 parts of eight bits each, which keep f32's exponent, so that no scale is shared
+// and nothing of one token or width touches another's bits; six of the nine part products run on the bf16 matrix instructions
+// with f32 sums, the other three being below f32's rounding.  Values are held as two f16 parts, hi and lo, after a scale by a
+// power of two that brings their tile's largest magnitude to [2^14, 2^15), probabilities the same way, from 2^14 down,
+// and three of four products are taken; value scales ride on the factor that rescales the output when a maximum moves.
+// A tile of 64 keys is split once for the whole block.
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
 // Measured: sixteen prompts of 256, four heads of 32: 14.0 us back to back (31 us with the f32 pipe); 16 x 1,024 tokens,
@@ -149,7 +149,7 @@ struct F32Shape {
   static constexpr int kRows = 16 * kWarps;
   static constexpr int kStride = D + 8;          // halves of a row in shared memory: rows apart by an odd number of 16 bytes
   static constexpr int kVecs = kKeys * D / 4 / kThreads;  // 16-byte words of a tile per thread
-  static constexpr int kBytes = 2 * (2 * kRows + 4 * kKeys) * kStride;
+  static constexpr int kBytes = 2 * (3 * kRows + 5 * kKeys) * kStride;
 };
 
 constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
@@ -159,6 +159,10 @@ __device__ __forceinline__ int split_exponent(float most) { return min(max(14 - 
 
 __device__ __forceinline__ unsigned pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned pack_bf162(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const unsigned*>(&h);
 }
 // pairs of floats in one 64-bit register
@@ -200,12 +204,30 @@ __device__ __forceinline__ uint2 split2(uint64_t x) {
   const float2 l = both(fma2(pair(h.x, h.y), pair(-1.f, -1.f), x));
   return make_uint2(hi, pack_half2(l.x, l.y));
 }
+// x in three bf16 parts of eight bits each, 24 together, which keep f32's exponent: the first is x cut off (a rounded
+// one could overflow), the others are rounded.  Of what is not finite the second and third are NaN.
+__device__ __forceinline__ uint3 split3(uint64_t x) {
+  float2 f = both(x);
+  uint3 p;
+  p.x = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+  x = fma2(pair(__uint_as_float(p.x << 16), __uint_as_float(p.x & 0xffff0000u)), pair(-1.f, -1.f), x);
+  f = both(x);
+  p.y = pack_bf162(f.x, f.y);
+  f = both(fma2(pair(__uint_as_float(p.y << 16), __uint_as_float(p.y & 0xffff0000u)), pair(-1.f, -1.f), x));
+  p.z = pack_bf162(f.x, f.y);
+  return p;
+}
+__device__ __forceinline__ void mma_bf16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_f16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void load_matrices(unsigned* r, const __half* at) {
+__device__ __forceinline__ void load_matrices(unsigned* r, const uint16_t* at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_addr(at))
@@ -234,13 +256,12 @@ template <int D>
 __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2 : 3) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
   using S = F32Shape<D>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __half* s_q = reinterpret_cast<__half*>(smem_raw);       // [2][kRows][kStride] hi, lo
-  __half* s_k = s_q + 2 * S::kRows * S::kStride;           // [2][kKeys][kStride]
-  __half* s_v = s_k + 2 * kKeys * S::kStride;              // [2][kKeys][kStride]
+  uint16_t* s_q = reinterpret_cast<uint16_t*>(smem_raw);                         // [3][kRows][kStride] bf16 parts
+  uint16_t* s_k = s_q + 3 * S::kRows * S::kStride;                               // [3][kKeys][kStride]
+  __half* s_v = reinterpret_cast<__half*>(s_k + 3 * kKeys * S::kStride);         // [2][kKeys][kStride] hi, lo
   __shared__ Tile s_tile;
-  __shared__ int2 s_most[S::kWarps];
+  __shared__ int s_most[S::kWarps];
   __shared__ int s_bad;
-  __shared__ int s_row[S::kRows];                          // scale exponents of the query rows
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = P.group, tile_tokens = S::kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
   const float* Q = static_cast<const float*>(P.q);
@@ -288,83 +309,67 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
         x[i] = __ldg(reinterpret_cast<const float4*>(Q + (t.begin + t.first + token) * P.q_token +
                                                      (static_cast<int64_t>(kv_head) * group + r % group) * P.q_head + d));
     }
+    // The scale is in the queries: scores less their maximum are then exact, where a product with the scale, rounded in the
+    // maximum alone, would put the weights of scores above 2^31 beyond the type.
+    const uint64_t scale = pair(P.scale_log2, P.scale_log2);
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
-      const int r = 16 * warp + i * kAtOnce + sub;
-      float most = 0.f;
-      const float e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (fabsf(e[u]) < INFINITY) most = fmaxf(most, fabsf(e[u]));
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-      const int scale = split_exponent(most);
-      const float up = P.scale_log2 < 0.f ? -pow2(scale) : pow2(scale);
-      if (d == 0) s_row[r] = scale;
-      const uint2 a = split2(pair(e[0] * up, e[1] * up)), b = split2(pair(e[2] * up, e[3] * up));
-      __half* to = s_q + r * S::kStride + d;
+      const uint3 a = split3(mul2(pair(x[i].x, x[i].y), scale)), b = split3(mul2(pair(x[i].z, x[i].w), scale));
+      uint16_t* to = s_q + (16 * warp + i * kAtOnce + sub) * S::kStride + d;
       *reinterpret_cast<uint2*>(to) = make_uint2(a.x, b.x);
       *reinterpret_cast<uint2*>(to + S::kRows * S::kStride) = make_uint2(a.y, b.y);
-      if (!(fabsf(e[0] + e[1] + e[2] + e[3]) < INFINITY)) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (!(fabsf(e[u]) < INFINITY)) to[S::kRows * S::kStride + u] = __float2half(0.f);
-      }
+      *reinterpret_cast<uint2*>(to + 2 * S::kRows * S::kStride) = make_uint2(a.z, b.z);
     }
   }
   __syncwarp();
   const int row0 = 16 * warp + g;  // this lane's rows: row0 and row0 + 8
   const int query0 = t.first + row0 / group, query1 = t.first + (row0 + 8) / group;  // their places in the sequence
-  const int sq0 = s_row[row0], sq1 = s_row[row0 + 8];
 
   float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   int unit = 0;  // the output is held times 2^(unit + 14)
-  const float scale = fabsf(P.scale_log2);
 
   for (int j0 = 0; j0 < last; j0 += kKeys) {
-    // the tile's scales, over the block
+    // the scale of the tile's values, over the block
     float mk = 0.f, mv = 0.f;
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
       mk = max3_nan(max3_nan(mk, fabsf(k[i].x), fabsf(k[i].y)), fabsf(k[i].z), fabsf(k[i].w));
       mv = max3_nan(max3_nan(mv, fabsf(v[i].x), fabsf(v[i].y)), fabsf(v[i].z), fabsf(v[i].w));
     }
-    const bool odd_k = !(mk < INFINITY), odd_v = !(mv < INFINITY);
-    if (odd_k || odd_v) {  // seldom: the largest of the finite ones, and values that are not finite are left out
+    const bool odd_k = !(mk < INFINITY);
+    if (!(mv < INFINITY)) {  // seldom: the largest of the finite ones, and values that are not finite are left out
       auto most_of = [](float most, float x) { return fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most; };
       auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
-      mk = mv = 0.f;
+      mv = 0.f;
 #pragma unroll
       for (int i = 0; i < S::kVecs; ++i) {
-        mk = most_of(most_of(most_of(most_of(mk, k[i].x), k[i].y), k[i].z), k[i].w);
         mv = most_of(most_of(most_of(most_of(mv, v[i].x), v[i].y), v[i].z), v[i].w);
         v[i] = make_float4(finite(v[i].x), finite(v[i].y), finite(v[i].z), finite(v[i].w));
       }
-      if (odd_v) s_bad = 1;
+      s_bad = 1;
     }
-    const int2 found = make_int2(__reduce_max_sync(kFull, __float_as_int(mk)), __reduce_max_sync(kFull, __float_as_int(mv)));
+    const int found = __reduce_max_sync(kFull, __float_as_int(mv));
     if (lane == 0) s_most[warp] = found;
     __syncthreads();  // also: the last tile is used up
-    int2 most = s_most[0];
+    int most = s_most[0];
 #pragma unroll
-    for (int w = 1; w < S::kWarps; ++w) most = make_int2(max(most.x, s_most[w].x), max(most.y, s_most[w].y));
-    const int ek = split_exponent(__int_as_float(most.x));
-    const int ev = most.y > 0 ? split_exponent(__int_as_float(most.y)) : unit;
-    const uint64_t uk = pair(pow2(ek), pow2(ek)), uv = pair(pow2(ev), pow2(ev));
+    for (int w = 1; w < S::kWarps; ++w) most = max(most, s_most[w]);
+    const int ev = most > 0 ? split_exponent(__int_as_float(most)) : unit;
+    const uint64_t uv = pair(pow2(ev), pow2(ev));
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
       const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
-      uint2 a = split2(mul2(pair(k[i].x, k[i].y), uk)), b = split2(mul2(pair(k[i].z, k[i].w), uk));
-      *reinterpret_cast<uint2*>(s_k + at) = make_uint2(a.x, b.x);
-      *reinterpret_cast<uint2*>(s_k + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
-      a = split2(mul2(pair(v[i].x, v[i].y), uv));
-      b = split2(mul2(pair(v[i].z, v[i].w), uv));
+      const uint3 x = split3(pair(k[i].x, k[i].y)), y = split3(pair(k[i].z, k[i].w));
+      *reinterpret_cast<uint2*>(s_k + at) = make_uint2(x.x, y.x);
+      *reinterpret_cast<uint2*>(s_k + kKeys * S::kStride + at) = make_uint2(x.y, y.y);
+      *reinterpret_cast<uint2*>(s_k + 2 * kKeys * S::kStride + at) = make_uint2(x.z, y.z);
+      const uint2 a = split2(mul2(pair(v[i].x, v[i].y), uv)), b = split2(mul2(pair(v[i].z, v[i].w), uv));
       *reinterpret_cast<uint2*>(s_v + at) = make_uint2(a.x, b.x);
       *reinterpret_cast<uint2*>(s_v + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
     }
-    if (odd_k) {  // what is not finite of a key meets hi parts of the queries alone: of a lo part 0 or of another sign it makes NaN
+    if (odd_k) {  // what is not finite of a key is its third part, which meets the queries' first alone: parts of unlike signs would make it NaN
 #pragma unroll
       for (int i = 0; i < S::kVecs; ++i) {
         const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
@@ -372,8 +377,8 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           if (!(fabsf(e[u]) < INFINITY)) {
-            s_k[at + u] = __float2half(0.f);
-            s_k[kKeys * S::kStride + at + u] = __float2half(e[u]);
+            s_k[at + u] = s_k[kKeys * S::kStride + at + u] = 0;
+            s_k[2 * kKeys * S::kStride + at + u] = static_cast<uint16_t>(pack_bf162(e[u], 0.f));
           }
       }
     }
@@ -385,31 +390,28 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 #pragma unroll
     for (int d = 0; d < D; d += 16) {
       if (d >= W) break;
-      unsigned qh[4], ql[4];
-      const __half* at = s_q + (16 * warp + (lane & 15)) * S::kStride + d + (lane >> 4) * 8;
-      load_matrices(qh, at);
-      load_matrices(ql, at + S::kRows * S::kStride);
+      unsigned q[3][4];
+      const uint16_t* at = s_q + (16 * warp + (lane & 15)) * S::kStride + d + (lane >> 4) * 8;
+#pragma unroll
+      for (int x = 0; x < 3; ++x) load_matrices(q[x], at + x * S::kRows * S::kStride);
 #pragma unroll
       for (int n = 0; n < 4; n += 2) {  // 32 keys: four sums take turns, as each product waits for the last of its sum
-        unsigned kh[8], kl[8];
+        unsigned b[3][8];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const __half* b = s_k + (16 * (n + x) + (lane & 7) + (lane >> 4) * 8) * S::kStride + d + (lane >> 3 & 1) * 8;
-          load_matrices(kh + 4 * x, b);
-          load_matrices(kl + 4 * x, b + kKeys * S::kStride);
+          const uint16_t* to = s_k + (16 * (n + x) + (lane & 7) + (lane >> 4) * 8) * S::kStride + d + (lane >> 3 & 1) * 8;
+#pragma unroll
+          for (int y = 0; y < 3; ++y) load_matrices(b[y] + 4 * x, to + y * kKeys * S::kStride);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], ql, kh[2 * x], kh[2 * x + 1]);
+        for (int y = 2; y >= 0; --y)  // products of parts y apart in all, the smallest first
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], qh, kl[2 * x], kl[2 * x + 1]);
+          for (int z = 0; z <= y; ++z)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(s[2 * n + x], qh, kh[2 * x], kh[2 * x + 1]);
+            for (int x = 0; x < 4; ++x) mma_bf16(s[2 * n + x], q[y - z], b[z][2 * x], b[z][2 * x + 1]);
       }
     }
     // softmax: columns 8 n + 2 c and the next of rows row0, row0 + 8
-    // factors of the scores, above 0 so that a masked one stays -inf (the scale's sign is in the queries)
-    const float f0 = fmaxf(pow2(min(max(-sq0 - ek, -126), 127)) * scale, kLeast);
-    const float f1 = fmaxf(pow2(min(max(-sq1 - ek, -126), 127)) * scale, kLeast);
     if (j0 + kKeys - 1 > t.first) {
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, x));
       big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, x));
     }
-    const float n0 = fmaxf(m0, big0 * f0), n1 = fmaxf(m1, big1 * f1);
+    const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
     const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;  // all -inf so far: weights 0
     float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
     m0 = n0;
@@ -451,11 +453,11 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     const float follow = step < -126 ? 0.f : pow2(step);
     a0 *= follow;
     a1 *= follow;
-    const uint64_t f00 = pair(f0, f0), f11 = pair(f1, f1), b00 = pair(-b0, -b0), b11 = pair(-b1, -b1);
+    const uint64_t b00 = pair(-b0, -b0), b11 = pair(-b1, -b1);
     uint64_t e0[8], e1[8], sum0 = pair(0.f, 0.f), sum1 = sum0;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const float2 y0 = both(fma2(pair(s[n][0], s[n][1]), f00, b00)), y1 = both(fma2(pair(s[n][2], s[n][3]), f11, b11));
+      const float2 y0 = both(add2(pair(s[n][0], s[n][1]), b00)), y1 = both(add2(pair(s[n][2], s[n][3]), b11));
       e0[n] = pair(exp2_fast(y0.x), exp2_fast(y0.y));
       e1[n] = pair(exp2_fast(y1.x), exp2_fast(y1.y));
       sum0 = add2(sum0, e0[n]);

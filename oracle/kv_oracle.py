@@ -137,3 +137,26 @@ def attend(q, k_rows, v_rows, scale=None) -> np.ndarray:
         for h in range(q.shape[1]):
             out[b, h] = softmax_rows(q[b, h][None], k_rows[b][:, h // group], v_rows[b][:, h // group], scale)[0]
     return out
+
+
+def prompt_with_bound(q, k, v, starts, scale=None):
+    """``prompt`` and how far float32 arithmetic may take each of its outputs, from that row's own sums.
+
+    A score is off by u of scale * sum_d |q_d k_d| and a weight p by that and u of itself, which moves the mean
+    o = sum p v by p |v - o| of it; the mean's products and sum take u of sum p |v|.  u = 2^-20: eight roundings."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    group = q.shape[1] // k.shape[1]
+    out, bound = np.full(q.shape, np.nan), np.zeros(q.shape)
+    for a, z in zip(starts[:-1], starts[1:]):
+        for h in range(q.shape[1]):
+            for i in range(a, z):
+                kk, vv = k[a:i + 1, h // group], v[a:i + 1, h // group]
+                s = scale * (kk @ q[i, h])
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                o = p @ vv
+                reach = abs(scale) * (np.abs(kk) @ np.abs(q[i, h]))
+                out[i, h] = o
+                bound[i, h] = 2.0**-20 * ((p * (reach + 1)) @ np.abs(vv - o) + p @ np.abs(vv))
+    return out, bound

@@ -98,3 +98,28 @@ def test_entry_points_reject_bad_arguments_without_a_gpu():
     assert prompt(width=136) == _lib.ERR_UNSUPPORTED
     assert prompt(width=36) == _lib.ERR_UNSUPPORTED
     assert prompt(heads=130) == _lib.ERR_UNSUPPORTED
+
+
+def test_the_float32_bound_tells_half_the_bits():
+    """Outputs whose queries and keys, values or weights were rounded to 11 bits lie outside it, float32 ones inside."""
+    rng = np.random.default_rng(0)
+    for length, width in ((60, 32), (120, 64), (90, 128)):
+        q, k, v = (rng.standard_normal((length, 1, width)).astype(np.float32) for _ in range(3))
+        want, bound = O.prompt_with_bound(q, k, v, [0, length])
+        np.testing.assert_allclose(want, O.prompt(q, k, v, [0, length]), rtol=1e-9, atol=1e-12)
+
+        def outside(q, k, v, weight=lambda p: p, t=np.float64):
+            got = np.zeros(want.shape)
+            for i in range(length):
+                s = (k[:i + 1, 0].astype(t) @ q[i, 0].astype(t)) * t(width**-0.5)
+                p = np.exp(s - s.max())
+                got[i, 0] = (weight(p).astype(t) @ v[:i + 1, 0].astype(t)) / p.sum()
+            return float((np.abs(got - want) > bound).mean())
+
+        def half(x):
+            return x.astype(np.float16).astype(np.float32)
+
+        assert outside(q, k, v, t=np.float32) == 0
+        assert outside(half(q), half(k), v) > 0.1
+        assert outside(q, k, half(v)) > 0.1
+        assert outside(q, k, v, weight=half) > 0.1
