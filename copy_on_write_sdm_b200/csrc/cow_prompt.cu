@@ -124,21 +124,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // f32
 // --------------------------------------------------------------------------
 //
-// Queries and keys are held as three bf16 parts of eight bits each, which keep f32's exponent, so that no scale is shared
-// and nothing of one token or width touches another's bits; six of the nine part products run on the bf16 matrix instructions
-// with f32 sums, the other three being below f32's rounding.  Values are held as two f16 parts, hi and lo, after a scale by a
-// power of two that brings their tile's largest magnitude to [2^14, 2^15), probabilities the same way, from 2^14 down,
-// and three of four products are taken; value scales ride on the factor that rescales the output when a maximum moves.
-// A tile of 64 keys is split once for the whole block.
+// Every operand is held as three bf16 parts of eight bits each, which keep f32's exponent: no scale is shared, and nothing
+// of one token, width or tile touches another's bits.  Six of the nine part products run on the bf16 matrix
+// instructions with f32 sums, the other three being below f32's rounding: f32's accuracy at a sixth of the 16-bit rate.
+// A tile of 64 keys is split once for the whole block.  Weights are 2^-8 at most, so that a sum of 256 of the
+// type's largest values does not overflow before its division; products below 2^-126 are lost to the matrix
+// instructions, so that values keep all 24 bits down to 2^-102 (2e-31).
 // Values that are not finite are left out of the products (a weight of 0 times them is NaN) and added at
 // the end to the rows that see them.
-// Measured: sixteen prompts of 256, four heads of 32: 14.0 us back to back (31 us with the f32 pipe); 16 x 1,024 tokens,
-// 32/8 heads of 128: 1.54 ms, 89 TFLOP/s of f32 work (266 of f16 products, of about 560 that `mma.sync` gives here:
-// 1,024 multiply-adds a cycle and SM).  Bound: the chain of split, scores, softmax and products of a key
-// tile, with two or three warps to a scheduler: a third of the issue slots and half of the matrix rate are in use.  What
-// shortened it was fewer instructions (packed pairs, rare cases on paths of their own: 1.69 -> 1.55 ms).  Tried
-// and not kept: two split tiles in turn with the next split beside the products, eight sums in turn instead of
-// four (no change); tiles of 32 keys (1.72 ms), four warps twice an SM (2.0 ms), 128 keys for width 32.
+// Measured: sixteen prompts of 256, four heads of 32: 16.4 us back to back (31 us with the f32 pipe); 16 x 1,024 tokens,
+// 32/8 heads of 128: 2.50 ms, 55 TFLOP/s of f32 work (330 of bf16 products, of about 560 that `mma.sync` gives here:
+// 1,024 multiply-adds a cycle and SM); error against 64 bits 0.5 to 0.8 of plain f32 sums'.  (Two f16 parts under scales
+// shared by a tile took 1.54 ms and were wrong wherever tokens of a tile lie far apart, those a row does not see among them.)
+// Bound: the matrix instructions, 60 % of their rate, and the chain of split, scores, softmax and products of a key
+// tile, with two or three warps to a scheduler.  Tried and not kept: all products of 16 widths in one go (2.43 ms, but
+// cut off 24 or 48 times instead of 4 or 8: four times the error for heads of 128); of the form with f16 parts: two split
+// tiles in turn with the next split beside the products, eight sums in turn instead of four (no change), tiles of 32 keys
+// (12 % slower), four warps twice an SM (30 %), 128 keys for width 32.
 
 constexpr int kKeys = 64;
 
@@ -149,18 +151,11 @@ struct F32Shape {
   static constexpr int kRows = 16 * kWarps;
   static constexpr int kStride = D + 8;          // halves of a row in shared memory: rows apart by an odd number of 16 bytes
   static constexpr int kVecs = kKeys * D / 4 / kThreads;  // 16-byte words of a tile per thread
-  static constexpr int kBytes = 2 * (3 * kRows + 5 * kKeys) * kStride;
+  static constexpr int kBytes = 2 * 3 * (kRows + 2 * kKeys) * kStride;
 };
 
 constexpr float kLeast = 1.1754943508222875e-38f;  // 2^-126
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
-// The exponent of the scale that brings `most` (finite, >= 0) to [2^14, 2^15), as far as both are normal.
-__device__ __forceinline__ int split_exponent(float most) { return min(max(14 - ((__float_as_int(most) >> 23) - 127), -113), 100); }
-
-__device__ __forceinline__ unsigned pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
+constexpr float kHeadroom = 8.f;                   // log2 of what weights lie below 1
 __device__ __forceinline__ unsigned pack_bf162(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const unsigned*>(&h);
@@ -196,14 +191,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// hi and lo parts of a and b, whose magnitudes are below 2^16; lo of what is not finite is NaN
-__device__ __forceinline__ uint2 split2(uint64_t x) {
-  const float2 f = both(x);
-  const unsigned hi = pack_half2(f.x, f.y);
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  const float2 l = both(fma2(pair(h.x, h.y), pair(-1.f, -1.f), x));
-  return make_uint2(hi, pack_half2(l.x, l.y));
-}
 // x in three bf16 parts of eight bits each, 24 together, which keep f32's exponent: the first is x cut off (a rounded
 // one could overflow), the others are rounded.  Of what is not finite the second and third are NaN.
 __device__ __forceinline__ uint3 split3(uint64_t x) {
@@ -222,18 +209,13 @@ __device__ __forceinline__ void mma_bf16(float* c, const unsigned* a, unsigned b
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16(float* c, const unsigned* a, unsigned b0, unsigned b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void load_matrices(unsigned* r, const uint16_t* at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_addr(at))
                : "memory");
 }
-__device__ __forceinline__ void load_matrices_turned(unsigned* r, const __half* at) {
+__device__ __forceinline__ void load_matrices_turned(unsigned* r, const uint16_t* at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_addr(at))
@@ -256,11 +238,10 @@ template <int D>
 __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2 : 3) cow_prompt_f32_kernel(const __grid_constant__ PromptLaunch P) {
   using S = F32Shape<D>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint16_t* s_q = reinterpret_cast<uint16_t*>(smem_raw);                         // [3][kRows][kStride] bf16 parts
-  uint16_t* s_k = s_q + 3 * S::kRows * S::kStride;                               // [3][kKeys][kStride]
-  __half* s_v = reinterpret_cast<__half*>(s_k + 3 * kKeys * S::kStride);         // [2][kKeys][kStride] hi, lo
+  uint16_t* s_q = reinterpret_cast<uint16_t*>(smem_raw);  // [3][kRows][kStride] bf16 parts
+  uint16_t* s_k = s_q + 3 * S::kRows * S::kStride;         // [3][kKeys][kStride]
+  uint16_t* s_v = s_k + 3 * kKeys * S::kStride;             // [3][kKeys][kStride]
   __shared__ Tile s_tile;
-  __shared__ int s_most[S::kWarps];
   __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = P.group, tile_tokens = S::kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
@@ -328,46 +309,33 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
   float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  int unit = 0;  // the output is held times 2^(unit + 14)
 
   for (int j0 = 0; j0 < last; j0 += kKeys) {
-    // the scale of the tile's values, over the block
-    float mk = 0.f, mv = 0.f;
+    float mk = 0.f, mv = 0.f;  // whether all of them are finite
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
       mk = max3_nan(max3_nan(mk, fabsf(k[i].x), fabsf(k[i].y)), fabsf(k[i].z), fabsf(k[i].w));
       mv = max3_nan(max3_nan(mv, fabsf(v[i].x), fabsf(v[i].y)), fabsf(v[i].z), fabsf(v[i].w));
     }
     const bool odd_k = !(mk < INFINITY);
-    if (!(mv < INFINITY)) {  // seldom: the largest of the finite ones, and values that are not finite are left out
-      auto most_of = [](float most, float x) { return fabsf(x) < INFINITY ? fmaxf(most, fabsf(x)) : most; };
+    if (!(mv < INFINITY)) {  // seldom: values that are not finite are left out
       auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
-      mv = 0.f;
 #pragma unroll
-      for (int i = 0; i < S::kVecs; ++i) {
-        mv = most_of(most_of(most_of(most_of(mv, v[i].x), v[i].y), v[i].z), v[i].w);
-        v[i] = make_float4(finite(v[i].x), finite(v[i].y), finite(v[i].z), finite(v[i].w));
-      }
+      for (int i = 0; i < S::kVecs; ++i) v[i] = make_float4(finite(v[i].x), finite(v[i].y), finite(v[i].z), finite(v[i].w));
       s_bad = 1;
     }
-    const int found = __reduce_max_sync(kFull, __float_as_int(mv));
-    if (lane == 0) s_most[warp] = found;
-    __syncthreads();  // also: the last tile is used up
-    int most = s_most[0];
-#pragma unroll
-    for (int w = 1; w < S::kWarps; ++w) most = max(most, s_most[w]);
-    const int ev = most > 0 ? split_exponent(__int_as_float(most)) : unit;
-    const uint64_t uv = pair(pow2(ev), pow2(ev));
+    __syncthreads();  // the last tile is used up
 #pragma unroll
     for (int i = 0; i < S::kVecs; ++i) {
       const int n = tid + i * S::kThreads, at = n / (D / 4) * S::kStride + 4 * (n % (D / 4));
-      const uint3 x = split3(pair(k[i].x, k[i].y)), y = split3(pair(k[i].z, k[i].w));
-      *reinterpret_cast<uint2*>(s_k + at) = make_uint2(x.x, y.x);
-      *reinterpret_cast<uint2*>(s_k + kKeys * S::kStride + at) = make_uint2(x.y, y.y);
-      *reinterpret_cast<uint2*>(s_k + 2 * kKeys * S::kStride + at) = make_uint2(x.z, y.z);
-      const uint2 a = split2(mul2(pair(v[i].x, v[i].y), uv)), b = split2(mul2(pair(v[i].z, v[i].w), uv));
-      *reinterpret_cast<uint2*>(s_v + at) = make_uint2(a.x, b.x);
-      *reinterpret_cast<uint2*>(s_v + kKeys * S::kStride + at) = make_uint2(a.y, b.y);
+      auto put = [&](uint16_t* to, float4 f) {
+        const uint3 a = split3(pair(f.x, f.y)), b = split3(pair(f.z, f.w));
+        *reinterpret_cast<uint2*>(to) = make_uint2(a.x, b.x);
+        *reinterpret_cast<uint2*>(to + kKeys * S::kStride) = make_uint2(a.y, b.y);
+        *reinterpret_cast<uint2*>(to + 2 * kKeys * S::kStride) = make_uint2(a.z, b.z);
+      };
+      put(s_k + at, k[i]);
+      put(s_v + at, v[i]);
     }
     if (odd_k) {  // what is not finite of a key is its third part, which meets the queries' first alone: parts of unlike signs would make it NaN
 #pragma unroll
@@ -385,30 +353,34 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     __syncthreads();
     if (j0 + kKeys < last) load(j0 + kKeys);
 
-    // scores: 16 rows x 64 keys
+    // Scores: 16 rows x 64 keys.  The matrix unit cuts sums off where f32 rounds them, so the small products are added up first
+    // and those of the first parts, which every later cut would be measured by, last.
     float s[8][4] = {};
 #pragma unroll
-    for (int d = 0; d < D; d += 16) {
-      if (d >= W) break;
-      unsigned q[3][4];
-      const uint16_t* at = s_q + (16 * warp + (lane & 15)) * S::kStride + d + (lane >> 4) * 8;
+    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-      for (int x = 0; x < 3; ++x) load_matrices(q[x], at + x * S::kRows * S::kStride);
+      for (int d = 0; d < D; d += 16) {
+        if (d >= W) break;
+        unsigned q[3][4];
+        const uint16_t* at = s_q + (16 * warp + (lane & 15)) * S::kStride + d + (lane >> 4) * 8;
 #pragma unroll
-      for (int n = 0; n < 4; n += 2) {  // 32 keys: four sums take turns, as each product waits for the last of its sum
-        unsigned b[3][8];
+        for (int y = 0; y < (pass ? 1 : 3); ++y) load_matrices(q[y], at + y * S::kRows * S::kStride);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint16_t* to = s_k + (16 * (n + x) + (lane & 7) + (lane >> 4) * 8) * S::kStride + d + (lane >> 3 & 1) * 8;
+        for (int n = 0; n < 4; n += 2) {  // 32 keys: four sums take turns, as each product waits for the last of its sum
+          unsigned b[3][8];
 #pragma unroll
-          for (int y = 0; y < 3; ++y) load_matrices(b[y] + 4 * x, to + y * kKeys * S::kStride);
+          for (int x = 0; x < 2; ++x) {
+            const uint16_t* to = s_k + (16 * (n + x) + (lane & 7) + (lane >> 4) * 8) * S::kStride + d + (lane >> 3 & 1) * 8;
+#pragma unroll
+            for (int y = 0; y < (pass ? 1 : 3); ++y) load_matrices(b[y] + 4 * x, to + y * kKeys * S::kStride);
+          }
+#pragma unroll
+          for (int y = pass ? 0 : 2; y >= (pass ? 0 : 1); --y)  // parts y apart in all
+#pragma unroll
+            for (int z = 0; z <= y; ++z)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) mma_bf16(s[2 * n + x], q[y - z], b[z][2 * x], b[z][2 * x + 1]);
         }
-#pragma unroll
-        for (int y = 2; y >= 0; --y)  // products of parts y apart in all, the smallest first
-#pragma unroll
-          for (int z = 0; z <= y; ++z)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) mma_bf16(s[2 * n + x], q[y - z], b[z][2 * x], b[z][2 * x + 1]);
       }
     }
     // softmax: columns 8 n + 2 c and the next of rows row0, row0 + 8
@@ -433,26 +405,13 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       big0 = fmaxf(big0, __shfl_xor_sync(kFull, big0, x));
       big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, x));
     }
-    const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
+    const float n0 = fmaxf(m0, big0 + kHeadroom), n1 = fmaxf(m1, big1 + kHeadroom);
     const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;  // all -inf so far: weights 0
-    float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
+    const float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
     m0 = n0;
     m1 = n1;
     l0 *= a0;
     l1 *= a1;
-    // The output follows the tile's value scale; a tile 2^64 below the others keeps theirs and its weights
-    // shrink instead, so no factor overflows.
-    if (j0 == 0) unit = ev;
-    int step = ev - unit;
-    float shrink = 1.f;
-    if (step > 64) {
-      shrink = pow2(max(-step, -126));
-      step = 0;
-    }
-    unit += step;
-    const float follow = step < -126 ? 0.f : pow2(step);
-    a0 *= follow;
-    a1 *= follow;
     const uint64_t b00 = pair(-b0, -b0), b11 = pair(-b1, -b1);
     uint64_t e0[8], e1[8], sum0 = pair(0.f, 0.f), sum1 = sum0;
 #pragma unroll
@@ -465,45 +424,49 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     }
     l0 += both(sum0).x + both(sum0).y;
     l1 += both(sum1).x + both(sum1).y;
-    const uint64_t up = pair(shrink * 16384.f, shrink * 16384.f);
-    unsigned ph[4][4], pl[4][4];  // by 16 keys
+    unsigned p[3][4][4];  // parts, by 16 keys
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      const uint2 u = split2(mul2(e0[n], up)), w = split2(mul2(e1[n], up));
-      ph[n / 2][2 * (n % 2)] = u.x;
-      ph[n / 2][2 * (n % 2) + 1] = w.x;
-      pl[n / 2][2 * (n % 2)] = u.y;
-      pl[n / 2][2 * (n % 2) + 1] = w.y;
+      const uint3 u = split3(e0[n]), w = split3(e1[n]);
+      p[0][n / 2][2 * (n % 2)] = u.x;
+      p[0][n / 2][2 * (n % 2) + 1] = w.x;
+      p[1][n / 2][2 * (n % 2)] = u.y;
+      p[1][n / 2][2 * (n % 2) + 1] = w.y;
+      p[2][n / 2][2 * (n % 2)] = u.z;
+      p[2][n / 2][2 * (n % 2) + 1] = w.z;
     }
 #pragma unroll
     for (int d = 0; d < D; d += 32) {
       if (d >= W) break;
       // The tile's sum apart, then added in f32: the matrix unit's own adds do not round to nearest, and over
       // a long prompt that would show.
-      float y[4][4] = {};
+      float y4[4][4] = {};
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        unsigned vh[8], vl[8];
+      for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const __half* b = s_v + (16 * n + (lane & 15)) * S::kStride + d + 16 * x + (lane >> 4) * 8;
-          load_matrices_turned(vh + 4 * x, b);
-          load_matrices_turned(vl + 4 * x, b + kKeys * S::kStride);
+        for (int n = 0; n < 4; ++n) {
+          unsigned b[3][8];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint16_t* at = s_v + (16 * n + (lane & 15)) * S::kStride + d + 16 * x + (lane >> 4) * 8;
+#pragma unroll
+            for (int y = 0; y < (pass ? 1 : 3); ++y) load_matrices_turned(b[y] + 4 * x, at + y * kKeys * S::kStride);
+          }
+#pragma unroll
+          for (int y = pass ? 0 : 2; y >= (pass ? 0 : 1); --y)
+#pragma unroll
+            for (int z = 0; z <= y; ++z)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) mma_bf16(y4[x], p[y - z][n], b[z][2 * x], b[z][2 * x + 1]);
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(y[x], pl[n], vh[2 * x], vh[2 * x + 1]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(y[x], ph[n], vl[2 * x], vl[2 * x + 1]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) mma_f16(y[x], ph[n], vh[2 * x], vh[2 * x + 1]);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         float* to = o[d / 8 + x];
-        to[0] = fmaf(to[0], a0, y[x][0]);
-        to[1] = fmaf(to[1], a0, y[x][1]);
-        to[2] = fmaf(to[2], a1, y[x][2]);
-        to[3] = fmaf(to[3], a1, y[x][3]);
+        to[0] = fmaf(to[0], a0, y4[x][0]);
+        to[1] = fmaf(to[1], a0, y4[x][1]);
+        to[2] = fmaf(to[2], a1, y4[x][2]);
+        to[3] = fmaf(to[3], a1, y4[x][3]);
       }
     }
   }
@@ -512,7 +475,6 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     l0 += __shfl_xor_sync(kFull, l0, x);
     l1 += __shfl_xor_sync(kFull, l1, x);
   }
-  const float down = pow2(min(max(-unit - 14, -126), 127));
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = row0 + 8 * half, token = r / group, query = half ? query1 : query0;
@@ -524,7 +486,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     for (int i = 0; i < D / 8; ++i) {
       const int d = 8 * i + 2 * c;
       if (d >= W) continue;
-      *reinterpret_cast<float2*>(out + d) = make_float2(o[i][2 * half] * down * inv, o[i][2 * half + 1] * down * inv);
+      *reinterpret_cast<float2*>(out + d) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
     }
     if (s_bad) add_nonfinite_f32(V + t.begin * P.v_token, P.v_token, query, out, 2 * c, W);
   }

@@ -20,6 +20,7 @@ def assert_within_own_sums(q, k, v, starts, device_starts, scale=None):
 
     got = _np(prompt_attention(q, k, v, device_starts, scale=scale))
     want, bound = O.prompt_with_bound(_np(q), _np(k), _np(v), starts, scale)
+    bound = bound + np.finfo(np.float32).tiny  # below it the type has no bits left to hold
     over = np.abs(got - want) - bound
     assert np.isfinite(got).all() and (over <= 0).all(), float(np.nanmax(np.abs(got - want) / np.maximum(bound, 1e-300)))
 
@@ -58,3 +59,54 @@ def test_keys_of_unlike_widths(dev, width):  # noqa: F811
     q, k = q / apart, k * apart
     q[..., 5], k[..., 5] = 0.0, 1e20
     assert_within_own_sums(q, k, v, starts, device_starts)
+
+
+@pytest.mark.parametrize("width", (32, 64, 128))
+@pytest.mark.parametrize("times", (1e6, 1e12, 1e30))
+def test_a_much_larger_value_changes_only_the_rows_that_see_it(dev, width, times):  # noqa: F811
+    q, k, v, starts, device_starts = _inputs(dev, [150, 40], 1, 2, width, torch.float32, 6)
+    v[[9, 100, 160]] *= times
+    assert_within_own_sums(q, k, v, starts, device_starts)
+
+
+@pytest.mark.parametrize("width", (32, 128))
+def test_a_much_larger_value_of_no_weight(dev, width):  # noqa: F811
+    """Every row sees it, with a weight of e^-300."""
+    q, k, v, starts, device_starts = _inputs(dev, [150, 40], 1, 2, width, torch.float32, 7)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[[0, 70, 150], :, 0] = -300 * width**0.5
+    v[[0, 70, 150]] *= 1e30
+    assert_within_own_sums(q, k, v, starts, device_starts)
+
+
+@pytest.mark.parametrize("width", (32, 64, 128))
+def test_values_of_unlike_widths(dev, width):  # noqa: F811
+    q, k, v, starts, device_starts = _inputs(dev, [150, 40], 1, 2, width, torch.float32, 8)
+    assert_within_own_sums(q, k, v * torch.logspace(-25, 25, width, device=dev), starts, device_starts)
+
+
+@pytest.mark.parametrize("sizes", [
+    (2.0**60, 1.0, 2.0**-60), (2.0**33, 2.0**-17, 2.0**-66), (1e4, 1e-12, 1e-26), (1e30, 1e10, 1e-10, 1e-30), (0.0, 1e-20, 1e-25),
+    (0.0, 0.0, 1e20, 1e-20), (1e-30, 1.0, 1e30), (1e30, 0.0, 1e-30),
+])
+@pytest.mark.parametrize("width", (32, 128))
+def test_values_that_fall_or_rise_from_tile_to_tile(dev, sizes, width):  # noqa: F811
+    """Also where the weight moves along with them: the second sequence's scores grow by hundreds from tile to tile, so
+    that the last tile's values alone are left."""
+    n = 64 * len(sizes)
+    q, k, v, starts, device_starts = _inputs(dev, [n, n], 1, 2, width, torch.float32, 9)
+    v *= torch.tensor(sizes * 2, device=dev).repeat_interleave(64)[:, None, None]
+    q[..., 0] = 1.0
+    k[n:, :, 0] = 400.0 * torch.arange(n, device=dev)[:, None].div(64, rounding_mode="floor") * width**0.5
+    assert_within_own_sums(q, k, v, starts, device_starts)
+
+
+def test_the_largest_values_of_the_type(dev):  # noqa: F811
+    """Means of numbers that would overflow if they were added up first (a little below the largest: a result rounded up
+    from that one is infinite)."""
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    q, k, v, starts, device_starts = _inputs(dev, [200], 1, 2, 32, torch.float32, 10)
+    v[:] = 0.99 * torch.finfo(torch.float32).min
+    got = prompt_attention(q, k, v, device_starts)
+    torch.testing.assert_close(got, torch.full_like(got, 0.99 * torch.finfo(torch.float32).min), rtol=2.0**-19, atol=0.0)
