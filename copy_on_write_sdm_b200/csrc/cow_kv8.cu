@@ -787,7 +787,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
         }
         big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
         big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
-        const int e = min(max(14 - exponent_of(big), -100), 100);
+        const int e = min(14 - exponent_of(big), 100);
         const float up = pow2(e), unscale = pow2(-e) * P.scale_log2;
 #pragma unroll
         for (int k = 0; k < S::kKeySteps; ++k) {

@@ -139,11 +139,20 @@ def attend(q, k_rows, v_rows, scale=None) -> np.ndarray:
     return out
 
 
-def prompt_with_bound(q, k, v, starts, scale=None):
-    """``prompt`` and how far float32 arithmetic may take each of its outputs, from that row's own sums.
-
-    A score is off by u of scale * sum_d |q_d k_d| and a weight p by that and u of itself, which moves the mean
+def _row_with_bound(q, k, v, scale):
+    """One query row against all of k, v [n, width], and how far float32 arithmetic may take each output, from the row's
+    own sums: a score is off by u of |scale| * sum_d |q_d k_jd| and a weight p by that and u of itself, which moves the mean
     o = sum p v by p |v - o| of it; the mean's products and sum take u of sum p |v|.  u = 2^-20: eight roundings."""
+    s = scale * (k @ q)
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    o = p @ v
+    reach = abs(scale) * (np.abs(k) @ np.abs(q))
+    return o, 2.0**-20 * ((p * (reach + 1)) @ np.abs(v - o) + p @ np.abs(v))
+
+
+def prompt_with_bound(q, k, v, starts, scale=None):
+    """``prompt`` and how far float32 arithmetic may take each of its outputs."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     scale = q.shape[2] ** -0.5 if scale is None else scale
     group = q.shape[1] // k.shape[1]
@@ -151,12 +160,17 @@ def prompt_with_bound(q, k, v, starts, scale=None):
     for a, z in zip(starts[:-1], starts[1:]):
         for h in range(q.shape[1]):
             for i in range(a, z):
-                kk, vv = k[a:i + 1, h // group], v[a:i + 1, h // group]
-                s = scale * (kk @ q[i, h])
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                o = p @ vv
-                reach = abs(scale) * (np.abs(kk) @ np.abs(q[i, h]))
-                out[i, h] = o
-                bound[i, h] = 2.0**-20 * ((p * (reach + 1)) @ np.abs(vv - o) + p @ np.abs(vv))
+                out[i, h], bound[i, h] = _row_with_bound(q[i, h], k[a:i + 1, h // group], v[a:i + 1, h // group], scale)
+    return out, bound
+
+
+def attend_with_bound(q, k_rows, v_rows, scale=None):
+    """``attend`` and how far float32 arithmetic may take each of its outputs."""
+    q = np.asarray(q, np.float64)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(q.shape[0]):
+        for h in range(q.shape[1]) if len(k_rows[b]) else ():
+            group = q.shape[1] // k_rows[b].shape[1]
+            out[b, h], bound[b, h] = _row_with_bound(q[b, h], k_rows[b][:, h // group], v_rows[b][:, h // group], scale)
     return out, bound
