@@ -384,8 +384,9 @@ __global__ void __launch_bounds__(kReadThreads) cow_kv8_read_kernel(const __grid
 //   contraction is 1/10 of what this instruction sustains at the memory's rate.
 //   Queries are scaled per head by a power of two into f16's range; f32 ones are
 //   held as two f16 parts (22 bits), and so are their probabilities.
-// * running maximum, sum and output of the softmax stay in f32 registers; value scales,
-//   powers of two, ride on the factor that rescales the output when the maximum moves.
+// * running maximum, sum and output of the softmax stay in f32 registers.  A page's weights are taken relative to its
+//   own largest score, so that f16 holds them whatever the others' are; the page's sums join the running ones in f32, where
+//   the difference of the maxima and the value scale are one factor.
 // Measured (32/8 heads of 128, bf16): 64 requests of 64 to 4,096 tokens 64 us (4.4 TB/s: 54 us of it the first kernel),
 // 4 of 65,536 102 us (5.3 TB/s, the first kernel 5.9); 16 of 256 to 512 tokens, 4 heads of 32, f32: 9.8 us, where
 // latency is all: 1.7 us until the lengths are scanned, 3.5 us for two pages, 1 us for the warps to meet.
@@ -400,6 +401,9 @@ constexpr int kJoinFewPairs = 148, kJoinThreadsFew = 512, kJoinThreadsMany = 128
 constexpr int kJoinColumns = 148 * 4;
 constexpr int kAlignedPages = 16;  // four pages a warp: less than a join through global memory takes
 constexpr float kProbShift = 8.f;  // probabilities are held times 2^8: more of f16's range below the largest
+// The output is held over 2^40: sums of the largest values do not overflow before their division, and the least
+// scale, 2^-64, leaves the smallest codes' products far above f32's last bit.
+constexpr float kOutUnit = 1099511627776.f, kOutUnitLog2 = 40.f;
 
 struct AttendLaunch {
   const uint8_t* key_codes;
@@ -549,6 +553,13 @@ struct Units {
   __device__ __forceinline__ int of(int x) const { return x < warps * first ? x / first : warps + (x - warps * first) / rest; }
 };
 
+// v + 2^x a, x a part's maximum less the largest: in two halves, as the weight may be below what f32 holds and the
+// part's output that far above the others'
+__device__ __forceinline__ float4 add_part(float x, float4 a, float4 v) {
+  const float half = exp2_fast(0.5f * x);
+  return f4_axpy(half, f4_scale(half, a), v);
+}
+
 template <int D, int kThreads>
 __device__ __forceinline__ void join_parts(const AttendLaunch& P, float (*s_ml)[2], float4 (*s_v)[D / 4], int u0, int sharers, int rows, int h,
                                            int64_t out_row) {
@@ -574,15 +585,14 @@ __device__ __forceinline__ void join_parts(const AttendLaunch& P, float (*s_ml)[
     float n = m;
 #pragma unroll
     for (int j = 0; j < kJoin; ++j) n = fmaxf(n, ml[j].x);
-    const float base = n == -INFINITY ? 0.f : n, fo = exp2_fast(m - base);
+    const float base = n == -INFINITY ? 0.f : n;
+    l *= exp2_fast(m - base);
+    v = add_part(m - base, v, make_float4(0.f, 0.f, 0.f, 0.f));
     m = n;
-    l *= fo;
-    v = f4_scale(fo, v);
 #pragma unroll
     for (int j = 0; j < kJoin; ++j) {
-      const float f = exp2_fast(ml[j].x - base);
-      l = fmaf(f, ml[j].y, l);
-      v = f4_axpy(f, a[j], v);
+      l = fmaf(exp2_fast(ml[j].x - base), ml[j].y, l);
+      v = add_part(ml[j].x - base, a[j], v);
     }
   }
   if (lane < kWords) s_v[warp][lane] = v;
@@ -600,11 +610,10 @@ __device__ __forceinline__ void join_parts(const AttendLaunch& P, float (*s_ml)[
     v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2_fast(s_ml[w][0] - base);
-      l = fmaf(f, s_ml[w][1], l);
-      v = f4_axpy(f, s_v[w][tid], v);
+      l = fmaf(exp2_fast(s_ml[w][0] - base), s_ml[w][1], l);
+      v = add_part(s_ml[w][0] - base, s_v[w][tid], v);
     }
-    st4_rt(P.out, out_row * D + 4 * tid, f4_scale(1.f / l, v), P.dtype);
+    st4_rt(P.out, out_row * D + 4 * tid, f4_scale(kOutUnit / l, v), P.dtype);
   }
   __syncthreads();  // the next pair's parts go there
 }
@@ -634,11 +643,10 @@ __device__ __forceinline__ void join_few(const AttendLaunch& P, int u0, int shar
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < kJoin; ++j) {
-      const float f = exp2_fast(ml[j].x - base);
-      l = fmaf(f, ml[j].y, l);
-      v = f4_axpy(f, a[j], v);
+      l = fmaf(exp2_fast(ml[j].x - base), ml[j].y, l);
+      v = add_part(ml[j].x - base, a[j], v);
     }
-    st4_rt(P.out, out_row * D + 4 * t, f4_scale(1.f / l, v), P.dtype);
+    st4_rt(P.out, out_row * D + 4 * t, f4_scale(kOutUnit / l, v), P.dtype);
   }
 }
 
@@ -760,7 +768,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
     unsigned qa[S::kKeySteps][2], qb[kSplit ? S::kKeySteps : 1][2];
     float f0 = 0.f, f1 = 0.f, m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
     float o[D / 16][4];
-    int ve = 0, length = 0;  // the output is held in units of 2^ve
+    int length = 0;
     bool fresh = true;
 
     for (int x = x0;;) {
@@ -805,7 +813,6 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
         l0 = l1 = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        ve = exponent_of(vs);
         fresh = false;
       }
 
@@ -895,40 +902,33 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
         big1 = fmaxf(big1, __shfl_xor_sync(kFull, big1, y));
       }
       const float n0 = fmaxf(m0, big0), n1 = fmaxf(m1, big1);
-      // where every score so far is -inf, exponents are taken from 0: probabilities 0, no NaN
-      const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-      float a0 = exp2_fast(m0 - b0), a1 = exp2_fast(m1 - b1);
+      // where every score of the page, or so far, is -inf, exponents are taken from 0: probabilities 0, no NaN
+      const float b0 = big0 == -INFINITY ? 0.f : big0, b1 = big1 == -INFINITY ? 0.f : big1;
+      const float c0 = n0 == -INFINITY ? 0.f : n0, c1 = n1 == -INFINITY ? 0.f : n1;
+      const float a0 = exp2_fast(m0 - c0), a1 = exp2_fast(m1 - c1), r0 = exp2_fast(big0 - c0), r1 = exp2_fast(big1 - c1);
       m0 = n0;
       m1 = n1;
-      l0 *= a0;
-      l1 *= a1;
-      // The output follows the page's value scale; a page 2^64 below the others keeps theirs and
-      // its probabilities shrink instead, so no factor overflows.
-      int step = ve - exponent_of(vs);
-      float shrink = 1.f;
-      if (step > 64) {
-        shrink = pow2(max(-step, -126));
-        step = 0;
-      }
-      ve -= step;
-      const float follow = step < -126 ? 0.f : pow2(step);
-      a0 *= follow;
-      a1 *= follow;
+      float sum0 = 0.f, sum1 = 0.f;
       unsigned pa[4][2], pb[kSplit ? 4 : 1][2];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const float e0 = exp2_fast(s[t][0] - b0 + kProbShift), e1 = exp2_fast(s[t][1] - b1 + kProbShift);
         const float e2 = exp2_fast(s[t][2] - b0 + kProbShift), e3 = exp2_fast(s[t][3] - b1 + kProbShift);
-        l0 += e0 + e2;
-        l1 += e1 + e3;
-        const unsigned u0 = pack_half2(e0 * shrink, e1 * shrink), u1 = pack_half2(e2 * shrink, e3 * shrink);
+        sum0 += e0 + e2;
+        sum1 += e1 + e3;
+        const unsigned u0 = pack_half2(e0, e1), u1 = pack_half2(e2, e3);
         pa[t][0] = transpose8x8(u0);
         pa[t][1] = transpose8x8(u1);
         if constexpr (kSplit) {
-          pb[t][0] = transpose8x8(pack_rest2(e0 * shrink, e1 * shrink, u0));
-          pb[t][1] = transpose8x8(pack_rest2(e2 * shrink, e3 * shrink, u1));
+          pb[t][0] = transpose8x8(pack_rest2(e0, e1, u0));
+          pb[t][1] = transpose8x8(pack_rest2(e2, e3, u1));
         }
       }
+      l0 = fmaf(l0, a0, sum0 * r0);
+      l1 = fmaf(l1, a1, sum1 * r1);
+      // one power of two for both: a page's weight may be below what f32 holds and its values that far above the others'
+      const float vs_log2 = static_cast<float>(exponent_of(vs)) - kOutUnitLog2;
+      const float y0 = exp2_fast(big0 - c0 + vs_log2), y1 = exp2_fast(big1 - c1 + vs_log2);
 
       if (!mbar_wait(&bars[1], parity, kSpinLimit) && lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
       parity ^= 1;
@@ -955,10 +955,10 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
           if constexpr (kSplit) mma_f16(y, v0, v1, v2, v3, pb[t][0], pb[t][1]);
           mma_f16(y, v0, v1, v2, v3, pa[t][0], pa[t][1]);
         }
-        o[i][0] = fmaf(o[i][0], a0, y[0]);
-        o[i][1] = fmaf(o[i][1], a1, y[1]);
-        o[i][2] = fmaf(o[i][2], a0, y[2]);
-        o[i][3] = fmaf(o[i][3], a1, y[3]);
+        o[i][0] = fmaf(o[i][0], a0, y[0] * y0);
+        o[i][1] = fmaf(o[i][1], a1, y[1] * y1);
+        o[i][2] = fmaf(o[i][2], a0, y[2] * y0);
+        o[i][3] = fmaf(o[i][3], a1, y[3] * y1);
       }
       if (more) {
         copy(1, next_tile);
@@ -974,11 +974,10 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
           l0 += __shfl_xor_sync(kFull, l0, y);
           l1 += __shfl_xor_sync(kFull, l1, y);
         }
-        const float scale = pow2(min(max(ve, -126), 127));
         const int chunk = now.pair % P.chunks, heads_here = min(kAttendHeads, P.group - chunk * kAttendHeads);
         const int64_t row = static_cast<int64_t>(now.b) * P.heads + now.pair / P.chunks * P.group + chunk * kAttendHeads;
         if (began && ended && !aligned) {
-          const float y0 = scale / l0, y1 = scale / l1;
+          const float y0 = kOutUnit / l0, y1 = kOutUnit / l1;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             if (2 * c < heads_here) {
@@ -996,12 +995,12 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             if (2 * c < rows) {
-              mine[(2 * c) * D + 16 * i + g] = o[i][0] * scale;
-              mine[(2 * c) * D + 16 * i + g + 8] = o[i][2] * scale;
+              mine[(2 * c) * D + 16 * i + g] = o[i][0];
+              mine[(2 * c) * D + 16 * i + g + 8] = o[i][2];
             }
             if (2 * c + 1 < rows) {
-              mine[(2 * c + 1) * D + 16 * i + g] = o[i][1] * scale;
-              mine[(2 * c + 1) * D + 16 * i + g + 8] = o[i][3] * scale;
+              mine[(2 * c + 1) * D + 16 * i + g] = o[i][1];
+              mine[(2 * c + 1) * D + 16 * i + g + 8] = o[i][3];
             }
           }
           if (g == 0) {
@@ -1050,12 +1049,11 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
       const float* part = reinterpret_cast<const float*>(smem + w * 2 * S::kBytes);
       const float2 ml = reinterpret_cast<const float2*>(part + rows * D)[h];
       const float n = fmaxf(m, ml.x), base = n == -INFINITY ? 0.f : n;
-      const float fo = exp2_fast(m - base), fr = exp2_fast(ml.x - base);
-      l = l * fo + ml.y * fr;
-      v = f4_axpy(fr, reinterpret_cast<const float4*>(part)[t], f4_scale(fo, v));
+      l = l * exp2_fast(m - base) + ml.y * exp2_fast(ml.x - base);
+      v = add_part(m - base, v, add_part(ml.x - base, reinterpret_cast<const float4*>(part)[t], make_float4(0.f, 0.f, 0.f, 0.f)));
       m = n;
     }
-    st4_rt(P.out, row * D + 4 * t, f4_scale(1.f / l, v), P.dtype);
+    st4_rt(P.out, row * D + 4 * t, f4_scale(kOutUnit / l, v), P.dtype);
   }
 }
 
