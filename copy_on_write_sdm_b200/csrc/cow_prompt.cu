@@ -538,6 +538,7 @@ constexpr int kTcKeys = 128;  // tokens of a key tile
 constexpr int kTcLimit = 1 << 18;                        // tries of the waits at a block's end
 constexpr unsigned long long kTcPatience = 2000000000ull;  // ns of the others
 constexpr float kLazy = 8.f;  // log2 of the growth of a maximum that is let pass
+constexpr float kFar = 16777216.f;  // half a last place of what is larger is 1 and more
 
 template <int DP>  // width rounded up to 32s
 struct TcShape {
@@ -1026,7 +1027,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
       if (t.count == 0) break;
       const int nx = x ? t.n_b : t.n_a;
       const int first = t.first + x * tile_tokens, query = first + row_token;  // its place in the sequence
-      float m = -INFINITY, l = 0.f;  // m: the maximum that P is relative to, the same in both halves
+      bool far = false;              // for any row of the warp: see kFar
+      float m = -INFINITY, l = 0.f;  // m: the score that P is relative to, the same in both halves
       for (int j = 0; j < nx; ++j, ++steps) {
         ok = __all_sync(kFull, wait(&bars.s[x], steps & 1)) && ok;
         tc_fence_after();
@@ -1048,15 +1050,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
           float& b = big[(i / 2) & 3];
           b = max3_nan(b, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
-        float now = max3_nan(max3_nan(big[0], big[1], big[2]), big[3], big[3]) * c;
-        if (any_of_two_warps(meet, !(now <= m + kLazy))) {  // NaN too
+        float now = max3_nan(max3_nan(big[0], big[1], big[2]), big[3], big[3]);
+        if (any_of_two_warps(meet, !((now - m) * c <= kLazy))) {  // NaN too
           s_most[x][half][row] = now;
           two_warps_meet(meet);
           now = max3_nan(now, s_most[x][half ^ 1][row], m);
-          const bool grown = !(now <= m + kLazy);
+          const bool grown = !((now - m) * c <= kLazy);
           float next = grown ? now : m;
           if (next == INFINITY) next = __int_as_float(0x7fc00000);  // inf - inf: the row is NaN, as any that sees one
-          const float a = next == -INFINITY ? 1.f : exp2_fast(m - next);
+          const float a = next == -INFINITY ? 1.f : exp2_fast((m - next) * c);
           m = next;
           l *= a;
           if (j > 0) {
@@ -1071,9 +1073,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
             }
             tc_wait_stores();
           }
+          far = __any_sync(kFull, row_token < tile_tokens && fabsf(m * c) > kFar && m != -INFINITY);
           two_warps_meet(meet);  // both have rescaled, and read the other's maximum
         }
-        const float base = m == -INFINITY ? 0.f : m;  // all -inf so far: weights 0
+        float base = m == -INFINITY ? 0.f : m * c;  // all -inf so far: weights 0
+        // The maximum times the scale is rounded, a score's product below is not: where that alone would drive weights out of
+        // range, the scores of the row are taken less their maximum first.  (From tensor memory, in few instructions.)
+        if (far) {
+          const int seen = query - j * kTcKeys - 64 * half;
+          const bool mine = fabsf(base) > kFar;
+          const float away = mine ? m : 0.f;
+#pragma unroll 1
+          for (int i = 0; i < 64; i += 8) {
+            unsigned r[8];
+            tc_load8(at_s + i, r);
+            tc_wait_loads();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) r[u] = i + u > seen ? 0xff800000u : __float_as_uint(__uint_as_float(r[u]) - away);
+            tc_store8(at_s + i, r);
+          }
+          tc_wait_stores();
+          tc_load32(at_s, s);
+          tc_load32(at_s + 32, s + 32);
+          tc_wait_loads();
+          if (mine) base = 0.f;
+        }
         const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
         uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll

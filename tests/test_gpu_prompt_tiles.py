@@ -1,5 +1,5 @@
 """Prompt attention where blocks take tile after tile, and with more sequences than a warp keeps in its registers,
-against the plain form in 64 bits on the same GPU.
+against the plain form in 64 bits on the same GPU; and 16-bit inputs near the ends of their types.
 
 Tolerance of an output, from its row's own sums: float32's bound (``oracle.kv_oracle.prompt_with_bound``), and for a type of
 unit roundoff u (2^-8 bfloat16, 2^-11 float16) 2 u of sum p |v|: the weight's rounding to the type (with float16's
@@ -86,3 +86,16 @@ def test_as_many_sequences_as_tokens(dev, dtype):  # noqa: F811
     q, k, v, _, device_starts = _inputs(dev, [1] * 1500, 2, 2, 32, dtype, 1)
     got = prompt_attention(q, k, v, device_starts)
     assert_within(got, v.double().repeat_interleave(2, 1), 2 * ROUNDOFF[dtype] * v.double().abs().repeat_interleave(2, 1) + 2.0**-20)
+
+
+@pytest.mark.parametrize("dtype,sizes", [(torch.bfloat16, (1e4, 1e10, 1e30)), (torch.float16, (3e2, 1e4))])
+@pytest.mark.parametrize("width", (64, 128))
+def test_much_larger_keys(dev, dtype, sizes, width):  # noqa: F811
+    """Scores far above 2^31: one token takes all the weight of the rows that see it, or none; the rows before it see the others."""
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    for size in sizes:
+        q, k, v, starts, device_starts = _inputs(dev, [200, 150], 1, 2, width, dtype, 21)
+        k[[9, 130, 220]] = (k[[9, 130, 220]].float() * size).to(dtype).clamp(torch.finfo(dtype).min, torch.finfo(dtype).max)
+        q[150:] = (q[150:].float() * 1e4).clamp(-6e4, 6e4).to(dtype)
+        assert_within(prompt_attention(q, k, v, device_starts), *plain(q, k, v, starts))
