@@ -540,12 +540,15 @@ constexpr unsigned long long kTcPatience = 2000000000ull;  // ns of the others
 constexpr float kLazy = 8.f;  // log2 of the growth of a maximum that is let pass
 constexpr float kFar = 16777216.f;  // half a last place of what is larger is 1 and more
 
-template <int DP>  // width rounded up to 32s
+template <int DT, int DP>  // DP: width rounded up to 32s
 struct TcShape {
   static constexpr int kParts = (DP + 63) / 64;                        // 128-byte wide parts of a row
   static constexpr int kPartBytes = 128 * 128;                  // 128 rows of one part
   static constexpr int kTileBytes = kParts * kPartBytes;
   static constexpr int kSlots = DP > 64 ? 4 : 8;                // ring of K and V tiles
+  // log2 of what weights lie below 1 (and up to kLazy above that): sums of bf16's largest values, which are f32's, do not
+  // overflow before their division; f16's do not come near, and its weights have no range to spare.
+  static constexpr float kUnder = DT == COW_BF16 ? 16.f : 0.f;
   static constexpr int kPoly = 2;                               // of 8 pairs of weights, those from the polynomial
   static constexpr int kStage = 16 * 1024;                      // 1 KB for each softmax warp: outputs on their way to rows
   static constexpr int kBytes = (2 + kSlots) * kTileBytes + kStage + 1024;
@@ -755,7 +758,7 @@ __device__ __noinline__ void add_nonfinite(const PromptLaunch& P, int first, int
 
 template <int DT, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __grid_constant__ TcLaunch L) {
-  using S = TcShape<DP>;
+  using S = TcShape<DT, DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcBarriers bars;
   __shared__ TcTile s_tiles[2];
@@ -1076,7 +1079,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
           far = __any_sync(kFull, row_token < tile_tokens && fabsf(m * c) > kFar && m != -INFINITY);
           two_warps_meet(meet);  // both have rescaled, and read the other's maximum
         }
-        float base = m == -INFINITY ? 0.f : m * c;  // all -inf so far: weights 0
+        float base = m == -INFINITY ? 0.f : fmaf(m, c, S::kUnder);  // all -inf so far: weights 0
         // The maximum times the scale is rounded, a score's product below is not: where that alone would drive weights out of
         // range, the scores of the row are taken less their maximum first.  (From tensor memory, in few instructions.)
         if (far) {
@@ -1096,7 +1099,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
           tc_load32(at_s, s);
           tc_load32(at_s + 32, s + 32);
           tc_wait_loads();
-          if (mine) base = 0.f;
+          if (mine) base = S::kUnder;
         }
         const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
         uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
@@ -1221,10 +1224,10 @@ bool encode_rows(CUtensorMap* map, int dtype, const void* base, int64_t tokens, 
 
 template <int DT, int DP>
 int launch_tc(const TcLaunch& L, unsigned blocks, cudaStream_t stream) {
-  const int resident = resident_blocks(reinterpret_cast<const void*>(cow_prompt_tc_kernel<DT, DP>), kTcThreads, TcShape<DP>::kBytes);
+  const int resident = resident_blocks(reinterpret_cast<const void*>(cow_prompt_tc_kernel<DT, DP>), kTcThreads, TcShape<DT, DP>::kBytes);
   if (!resident) return COW_ERR_CUDA;
   const unsigned grid = blocks < static_cast<unsigned>(resident) ? blocks : static_cast<unsigned>(resident);
-  cow_prompt_tc_kernel<DT, DP><<<grid, kTcThreads, TcShape<DP>::kBytes, stream>>>(L);
+  cow_prompt_tc_kernel<DT, DP><<<grid, kTcThreads, TcShape<DT, DP>::kBytes, stream>>>(L);
   return launch_status();
 }
 

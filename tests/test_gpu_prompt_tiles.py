@@ -99,3 +99,13 @@ def test_much_larger_keys(dev, dtype, sizes, width):  # noqa: F811
         k[[9, 130, 220]] = (k[[9, 130, 220]].float() * size).to(dtype).clamp(torch.finfo(dtype).min, torch.finfo(dtype).max)
         q[150:] = (q[150:].float() * 1e4).clamp(-6e4, 6e4).to(dtype)
         assert_within(prompt_attention(q, k, v, device_starts), *plain(q, k, v, starts))
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_the_largest_values_of_the_type(dev, dtype):  # noqa: F811
+    """Means of numbers whose sums lie beyond float32."""
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    q, k, v, starts, device_starts = _inputs(dev, [300], 1, 2, 64, dtype, 22)
+    v[:] = 0.98 * torch.finfo(dtype).min
+    assert_within(prompt_attention(q, k, v, device_starts), *plain(q, k, v, starts))
