@@ -15,7 +15,7 @@ from .allocator import (
     packed_sdm_cow_step,
     packed_sdm_cow_step_layers,
 )
-from .kv_cache import PagedKVCache, PagePlan, prompt_attention
+from .kv_cache import PagedKVCache, PagePlan, prompt_attention, prompt_attention_status
 from .session import DecodeSession
 
 __all__ = [
@@ -29,4 +29,5 @@ __all__ = [
     "packed_sdm_cow_step",
     "packed_sdm_cow_step_layers",
     "prompt_attention",
+    "prompt_attention_status",
 ]

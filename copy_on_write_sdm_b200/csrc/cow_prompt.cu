@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 // through only where some row does not see them, and from a step earlier (no change).
 // Of eight pairs of weights, two come from the polynomial (0: 395,000 cycles for 8,192 tokens of
 // 16/4 heads of 64, 2: 354,000, 3: 369,000).
-// Every wait is bounded; one that gives up sets a status bit and ends the block, its current rows NaN.
+// Every wait is bounded; one that gives up sets a status bit and ends the block, all its rows NaN.
 
 constexpr int kTcThreads = 640;
 constexpr int kTcRows = 128;  // rows of a tile
@@ -756,6 +756,27 @@ __device__ __noinline__ void add_nonfinite(const PromptLaunch& P, int first, int
   }
 }
 
+// What a block works on at place i of its own order: back and forth over the blocks, so that each gets large and small tiles.
+__device__ __forceinline__ int place_of(int i) { return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+
+// A wait gave up: every row of the block's tiles becomes NaN, those it had not come to among them.  By all warps.
+__device__ __noinline__ void give_up_rows(const PromptLaunch& P, int tile_tokens) {
+  const int lane = threadIdx.x & 31;
+  TileFinder finder;
+  finder.begin(P, tile_tokens);
+  for (int i = threadIdx.x >> 5;; i += kTcThreads / 32) {
+    const int w = place_of(i);
+    const Tile t = finder.find(P, tile_tokens, w / P.kv_heads);
+    if (t.count == 0) return;
+    const int row = P.group * P.width, here = min(tile_tokens, t.count - t.first);
+    for (int token = 0; token < here; ++token) {
+      uint16_t* out = static_cast<uint16_t*>(P.out) +
+                      (static_cast<int64_t>(t.begin + t.first + token) * P.heads + static_cast<int64_t>(w % P.kv_heads) * P.group) * P.width;
+      for (int d = lane; d < row; d += 32) out[d] = 0x7fff;  // NaN in either type
+    }
+  }
+}
+
 template <int DT, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __grid_constant__ TcLaunch L) {
   using S = TcShape<DT, DP>;
@@ -817,12 +838,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   };
 
   if (warp == 19) {
-    // ---- what to work on: tiles in the order of their work, back and forth over the blocks so that
-    // each gets large and small ones
+    // ---- what to work on: tiles in the order of their work
     TileFinder finder;
     finder.begin(P, 2 * tile_tokens);
     for (int i = 0;; ++i) {
-      const int w = i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      const int w = place_of(i);
       const Tile f = finder.find(P, 2 * tile_tokens, w / P.kv_heads);
       if (i >= 2 && !__all_sync(kFull, wait(&bars.tile_empty[i & 1], ((i >> 1) - 1) & 1))) break;
       if (lane == 0) {
@@ -1187,7 +1207,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) cow_prompt_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
-  if (tid == 0 && s_abort && P.status) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+  if (s_abort) {
+    if (tid == 0 && P.status) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+    give_up_rows(P, 2 * tile_tokens);
+  }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -36,6 +36,7 @@ _STATUS_TEXT = [
     (_lib.ST_INDEX_RANGE, "a request's length lies outside its block table"),
     (_lib.ST_PLAN_TOKENS, "a resize adds more tokens than were announced"),
     (_lib.ST_ROW_RANGE, "a block table holds no page for a cached token"),
+    (_lib.ST_WAIT_TIMEOUT, "a bounded wait in an attention kernel gave up: the rows it was for are NaN"),
 ]
 
 
@@ -80,8 +81,8 @@ _PROMPT_STATUS: dict[int, torch.Tensor] = {}
 
 
 def prompt_attention_status(device: torch.device) -> torch.Tensor:
-    """The device's status word of ``prompt_attention``: 0, or ``_lib.ST_WAIT_TIMEOUT`` once a
-    wait inside the kernel gave up and left rows unwritten."""
+    """The device's status word of ``prompt_attention`` calls without one of their own: 0, or ``_lib.ST_WAIT_TIMEOUT`` once a
+    wait inside the kernel gave up and made rows NaN.  Who reads it may zero it."""
     word = _PROMPT_STATUS.get(device.index)
     if word is None:
         word = _PROMPT_STATUS[device.index] = torch.zeros((), dtype=torch.int32, device=device)
@@ -89,7 +90,7 @@ def prompt_attention_status(device: torch.device) -> torch.Tensor:
 
 
 def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, starts: torch.Tensor, *,
-                     scale: float | None = None) -> torch.Tensor:
+                     scale: float | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention over packed prompts.
 
     ``queries`` ``[tokens, heads, width]``, ``keys`` and ``values`` ``[tokens, kv_heads,
@@ -98,6 +99,10 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     attends to its own sequence's tokens up to itself with ``softmax(scale * q . k)``, ``scale``
     1 / sqrt(width) by default; ``heads / kv_heads`` neighbouring query heads share a key head.
     Returns ``[tokens, heads, width]``; rows of tokens outside every sequence are unspecified.
+
+    Sums and softmax statistics are float32; 16-bit inputs have their weights rounded to their type before
+    they meet the values.  ``status`` (an int32 device word, a cache's ``status_word`` for one; ``prompt_attention_status``
+    by default) collects a wait that gave up, whose rows are NaN.
     """
     if queries.ndim != 3 or keys.ndim != 3 or keys.shape != values.shape:
         raise ValueError("prompt attention takes queries, keys and values [tokens, heads, width]")
@@ -116,9 +121,13 @@ def prompt_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
         raise ValueError("queries, keys, values and starts must be on one device")
     if starts.dtype != torch.int32 or starts.ndim != 1 or starts.numel() < 1 or not starts.is_contiguous():
         raise ValueError("starts must be a contiguous int32 vector [sequences + 1]")
+    if status is None:
+        status = prompt_attention_status(device)
+    elif status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+        raise ValueError("status must be one int32 on the inputs' device")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _call(device, "cow_prompt_attention", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, starts.data_ptr(), starts.numel() - 1, tokens, heads, kv_heads, width,
-          code, width ** -0.5 if scale is None else float(scale), out.data_ptr(), prompt_attention_status(device).data_ptr())
+          code, width ** -0.5 if scale is None else float(scale), out.data_ptr(), status.data_ptr())
     return out
 
 

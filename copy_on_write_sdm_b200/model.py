@@ -72,9 +72,10 @@ class CausalSelfAttention(nn.Module):
         return qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
 
     def prefill_packed(self, tokens: torch.Tensor, plan: "PagePlan", cache: "PagedKVCache", *, layer: int) -> torch.Tensor:
-        """Whole prompts of a plan's requests, packed ``[tokens, width]``; their K/V go to the cache."""
+        """Whole prompts of a plan's requests, packed ``[tokens, width]``; their K/V go to the cache, and
+        device errors to its status word."""
         q, k, v = self._project_packed(tokens)
-        attended = prompt_attention(q, k, v, plan.starts)
+        attended = prompt_attention(q, k, v, plan.starts, status=cache.status_word)
         cache.store(k, v, plan, layer=layer)
         return self.output(attended.view(-1, self.width))
 

@@ -161,6 +161,14 @@ class PagedServing:
         if not keep:
             self.sdm = None
 
+    def validate_invariants(self) -> None:
+        """Raise on any device error so far, of attention or of the pools, and where pages or rows are lost (synchronises)."""
+        self.cache.validate_invariants()
+        for state in () if self.sdm is None else self.sdm.sdm_states:
+            state.validate_invariants()
+        if self.cache.lengths.tolist() != self.lengths:
+            raise AssertionError("the K/V cache's lengths are not the requests'")
+
     def storage_bytes(self) -> dict[str, int]:
         """The SDM state's bytes (``FaithfulSDMDecodeState``'s keys) and the K/V cache's."""
         sdm = {} if self.sdm is None else self.sdm.storage_bytes()

@@ -55,9 +55,7 @@ def main() -> None:
             next_ids = torch.cat((next_ids[kept], logits.argmax(-1)))
     torch.cuda.synchronize()
     seconds = time.perf_counter() - began
-    serving.cache.validate_invariants()
-    for state in serving.sdm.sdm_states:
-        state.validate_invariants()
+    serving.validate_invariants()
     print(f"{decoded} tokens in {seconds:.2f} s, {named} requests served, lengths now {min(serving.lengths)} to {max(serving.lengths)}, "
           f"{serving.free_pages} of {serving.cache.pages} K/V pages free")
 

@@ -639,7 +639,7 @@ int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries
  * contiguous.  width a multiple of 8 up to 128, heads a multiple of kv_heads
  * with at most 64 query heads to a key head.  Tokens outside every sequence
  * are not written.  status (a device word, may be NULL) gets
- * COW_ST_WAIT_TIMEOUT if a wait inside a block gave up; rows are then missing. */
+ * COW_ST_WAIT_TIMEOUT if a wait inside a block gave up; that block's rows are then NaN. */
 int cow_prompt_attention(const void* queries, int64_t query_token_stride, int64_t query_head_stride,
                          const void* keys, int64_t key_token_stride, int64_t key_head_stride, const void* values,
                          int64_t value_token_stride, int64_t value_head_stride, const int32_t* starts,

@@ -1,0 +1,64 @@
+"""What the attention layers' operators report of errors on the device, and what they refuse on the host.  The words are
+set by hand: no test makes a kernel's wait run out."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_gpu_kv_cache import _cache, dev  # noqa: F401
+from tests.test_gpu_paged_serving import _model, _prompts
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_wait_that_gave_up_is_raised_by_name(dev):  # noqa: F811
+    from copy_on_write_sdm_b200 import _lib
+
+    cache = _cache(dev, requests=1, pages=1, kv_heads=1, head_width=32, max_blocks=1)
+    cache.status_word.fill_(_lib.ST_WAIT_TIMEOUT)
+    with pytest.raises(RuntimeError, match="wait .* gave up"):
+        cache.validate_invariants()
+
+
+def test_prompts_report_to_the_word_they_are_given(dev, monkeypatch):  # noqa: F811
+    from copy_on_write_sdm_b200 import kv_cache, prompt_attention, prompt_attention_status
+
+    words, call = [], kv_cache._call
+
+    def watched(device, what, *args):
+        if what == "cow_prompt_attention":
+            words.append(args[-1])
+        call(device, what, *args)
+
+    monkeypatch.setattr(kv_cache, "_call", watched)
+    x = torch.randn(5, 2, 32, device=dev)
+    starts = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    word = torch.zeros(1, dtype=torch.int32, device=dev)
+    prompt_attention(x, x, x, starts)
+    prompt_attention(x, x, x, starts, status=word)
+    assert words == [prompt_attention_status(dev).data_ptr(), word.data_ptr()] and not word.item()
+    for bad in (word.long(), word.cpu(), torch.zeros(2, dtype=torch.int32, device=dev)):
+        with pytest.raises(ValueError):
+            prompt_attention(x, x, x, starts, status=bad)
+
+
+def test_serving_reports_attention_errors(dev, monkeypatch):  # noqa: F811
+    from copy_on_write_sdm_b200 import _lib, kv_cache
+    from copy_on_write_sdm_b200.paged import PagedServing
+
+    words, call = [], kv_cache._call
+
+    def watched(device, what, *args):
+        if what == "cow_prompt_attention":
+            words.append(args[-1])
+        call(device, what, *args)
+
+    monkeypatch.setattr(kv_cache, "_call", watched)
+    serving = PagedServing(_model(dev, "BA"), pages=6, sdm_growth_quantum_rows=64)
+    serving.admit(_prompts([5, 70], 0), ["a", "b"])
+    assert words == [serving.cache.status_word.data_ptr()]
+    serving.validate_invariants()
+    serving.cache.status_word.fill_(_lib.ST_WAIT_TIMEOUT)
+    with pytest.raises(RuntimeError, match="gave up"):
+        serving.validate_invariants()
