@@ -770,6 +770,16 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
     float o[D / 16][4];
     int length = 0;
     bool fresh = true;
+    // A wait that gave up is reported; what is on its way gets as long again, no copy follows it, and the warp's
+    // outputs from there on are NaN.
+    bool lost = false;
+    auto wait = [&](int which, unsigned phase, bool next_keys) {
+      if (lost || __all_sync(kFull, mbar_wait(&bars[which], phase, kSpinLimit))) return;
+      lost = true;
+      if (lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+      if (!which || next_keys) mbar_wait(&bars[0], which ? phase ^ 1 : phase, kSpinLimit);
+      mbar_wait(&bars[1], phase, kSpinLimit);
+    };
 
     for (int x = x0;;) {
       if (fresh) {
@@ -848,8 +858,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
         }
       }
 
-      // A wait that gives up is reported and the page taken as it is.
-      if (!mbar_wait(&bars[0], parity, kSpinLimit) && lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+      wait(0, parity, false);
       float s[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -880,7 +889,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
           }
         }
       }
-      if (more) copy(0, next_tile);
+      if (more && !lost) copy(0, next_tile);
 
       // scores, the page's maximum, probabilities
       const int left = length - now.p * kPage;  // tokens of this page, if below 64
@@ -930,7 +939,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
       const float vs_log2 = static_cast<float>(exponent_of(vs)) - kOutUnitLog2;
       const float y0 = exp2_fast(big0 - c0 + vs_log2), y1 = exp2_fast(big1 - c1 + vs_log2);
 
-      if (!mbar_wait(&bars[1], parity, kSpinLimit) && lane == 0) atomicOr(P.status, COW_ST_WAIT_TIMEOUT);
+      wait(1, parity, more);
       parity ^= 1;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
@@ -961,7 +970,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
         o[i][3] = fmaf(o[i][3], a1, y[3] * y1);
       }
       if (more) {
-        copy(1, next_tile);
+        if (!lost) copy(1, next_tile);
         ks = P.key_scales[next_tile];
         vs = P.value_scales[next_tile];
       }
@@ -974,6 +983,7 @@ __global__ void __launch_bounds__(kAttendThreads, D > 64 ? 3 : 4) cow_kv8_attend
           l0 += __shfl_xor_sync(kFull, l0, y);
           l1 += __shfl_xor_sync(kFull, l1, y);
         }
+        if (lost) l0 = l1 = __int_as_float(0x7fc00000);
         const int chunk = now.pair % P.chunks, heads_here = min(kAttendHeads, P.group - chunk * kAttendHeads);
         const int64_t row = static_cast<int64_t>(now.b) * P.heads + now.pair / P.chunks * P.group + chunk * kAttendHeads;
         if (began && ended && !aligned) {

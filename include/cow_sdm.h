@@ -623,8 +623,8 @@ int cow_kv8_read(const cow_kv_pages* cache, int32_t layer, const int32_t* slots,
  * cow_kv8_attend_workspace_bytes bytes (-1: bad arguments), the same for any
  * number of requests, 16-byte aligned, its first 16 bytes zero before its first
  * use, and left ready for the next call; calls that may overlap on the GPU need
- * separate ones.  A bounded wait that gives up sets COW_ST_WAIT_TIMEOUT, a
- * table without a page for a cached token COW_ST_ROW_RANGE. */
+ * separate ones.  A bounded wait that gives up sets COW_ST_WAIT_TIMEOUT (the
+ * outputs that it was for are NaN), a table without a page for a cached token COW_ST_ROW_RANGE. */
 int64_t cow_kv8_attend_workspace_bytes(const cow_kv_pages* cache, int32_t heads);
 int cow_kv8_attend(const cow_kv_pages* cache, int32_t layer, const void* queries, int64_t query_request_stride,
                    int64_t query_head_stride, int32_t dtype, int32_t heads, float scale, void* out, void* workspace,
