@@ -26,6 +26,9 @@ class PagedServing:
     ``requests`` lists the live requests' names in batch order; ids go in and logits
     come out in that order.  ``pages`` is the K/V pool's size in pages of 64 tokens, shared by
     all requests; one page holds 64 tokens of every attention layer.
+
+    An ``admit`` that raises leaves the batch as it was.  A ``decode`` or ``release`` that raises on its way through the
+    layers does not, as the pools have taken some of its writes: every later call then raises ``RuntimeError``.
     """
 
     def __init__(self, model: LanguageModel, *, pages: int, sdm_growth_quantum_rows: int = 1024) -> None:
@@ -38,6 +41,7 @@ class PagedServing:
         self.requests: list[object] = []
         self.lengths: list[int] = []
         self.sdm: FaithfulSDMDecodeState | None = None
+        self._unusable: str | None = None
         attention = [stack.attention_layers[str(i)].attention for i, kind in enumerate(stack.layout) if kind == "A"]
         if not attention:
             raise ValueError("paged serving is for models with attention layers")
@@ -51,10 +55,23 @@ class PagedServing:
         """Free K/V pages, from the host's record of the lengths."""
         return self.cache.pages - sum(-(-n // PAGE_TOKENS) for n in self.lengths)
 
+    def _check_usable(self) -> None:
+        if self._unusable is not None:
+            raise RuntimeError(f"paged serving is unusable: {self._unusable} failed part way")
+
+    def _ids(self, ids: torch.Tensor) -> torch.Tensor:
+        """Token ids on the model's device; those on the host are checked, as one outside the vocabulary faults there."""
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError("token ids must be int32 or int64")
+        if not ids.is_cuda and ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.model.token_embedding.num_embeddings:
+            raise ValueError("token ids lie outside the vocabulary")
+        return ids.to(self.cache.device)
+
     @torch.no_grad()
     def admit(self, prompts: Sequence[torch.Tensor], names: Sequence[object]) -> torch.Tensor:
         """Prefill prompts (vectors of ids, any lengths) and add them to the batch, ordered by
         length after the live requests; the logits after each prompt's last token, in batch order."""
+        self._check_usable()
         if len(prompts) != len(names) or len(set(names)) != len(names) or set(names) & set(self.requests):
             raise ValueError("admitted requests need one new name each")
         if not prompts:
@@ -65,11 +82,32 @@ class PagedServing:
         counts = [prompts[i].shape[0] for i in order]
         if sum(-(-n // PAGE_TOKENS) for n in counts) > self.free_pages:
             raise ValueError("the K/V cache has too few free pages for the admitted prompts")
-        model, stack, device = self.model, self.model.stack, self.cache.device
-        live = len(self.requests)
-        self.cache = self.cache.with_requests(torch.arange(live, device=device), new=len(counts))
+        ids = torch.cat([self._ids(prompts[i]) for i in order])
+        live, cache, sdm = len(self.requests), self.cache, self.sdm
+        try:
+            logits = self._admit(ids, counts, live)
+        except BaseException:
+            self._unusable = "an admission and its undoing"
+            if self.cache is not cache:  # pages and rows taken so far go back
+                self.cache.resize(self.lengths + [0] * len(counts), tokens=0)
+                self.cache = self.cache.with_requests(torch.arange(live, device=cache.device))
+            self.sdm = sdm
+            if sdm is not None:
+                if sdm.batch > live:
+                    sdm.release_and_compact(list(range(live, sdm.batch)))
+                heads = [self.model.stack.sdm_layers[str(i)].memory_heads for i in sdm.sdm_layer_positions]
+                if [state.banks for state in sdm.sdm_states] != [live * h for h in heads]:
+                    raise
+            self._unusable = None
+            raise
+        self.requests += [names[i] for i in order]
+        self.lengths += counts
+        return logits
+
+    def _admit(self, ids: torch.Tensor, counts: list[int], live: int) -> torch.Tensor:
+        model, stack = self.model, self.model.stack
+        self.cache = self.cache.with_requests(torch.arange(live, device=self.cache.device), new=len(counts))
         plan = self.cache.resize(self.lengths + counts, tokens=sum(counts))
-        ids = torch.cat([prompts[i] for i in order]).to(device)
         tokens = model._embed(ids, plan.positions.long())
 
         groups: list[tuple[int, int, int]] = []  # first token, requests, length
@@ -101,30 +139,38 @@ class PagedServing:
         for (_, many, n), kept in zip(groups, pools):
             cohort = FaithfulSDMDecodeState(
                 layout=stack.layout, position=n, capacity=model.maximum_sequence_length, activation_dtype=tokens.dtype,
-                active_sequences=torch.ones(many, device=device, dtype=torch.bool), sdm_layer_positions=b_layers,
+                active_sequences=torch.ones(many, device=ids.device, dtype=torch.bool), sdm_layer_positions=b_layers,
                 sdm_states=tuple(kept), dense_keys=(), dense_values=())
             if self.sdm is None:
                 self.sdm = cohort
             else:
                 self.sdm.admit(cohort)
-        self.requests += [names[i] for i in order]
-        self.lengths += counts
         ends = plan.starts[live + 1:].long() - 1
         return model.output(model.final_norm(tokens[ends]))
 
     @torch.no_grad()
     def decode(self, ids: torch.Tensor) -> torch.Tensor:
         """One more token of every live request, ``[requests]`` ids to ``[requests, vocabulary]`` logits."""
+        self._check_usable()
         count = len(self.requests)
         if ids.shape != (count,) or count == 0:
             raise ValueError(f"decode ids must be [{count}], one for each live request")
-        model, stack = self.model, self.model.stack
+        model = self.model
         if max(self.lengths) >= model.maximum_sequence_length:
             raise ValueError("sequence exceeds maximum_sequence_length")
         if sum(n % PAGE_TOKENS == 0 for n in self.lengths) > self.free_pages:
             raise ValueError("the K/V cache has too few free pages for the next token")
+        ids = self._ids(ids)
+        self._unusable = "a decode step"
+        tokens = self._decode(ids, count)
+        self._unusable = None
+        self.lengths = [n + 1 for n in self.lengths]
+        return model.output(model.final_norm(tokens))
+
+    def _decode(self, ids: torch.Tensor, count: int) -> torch.Tensor:
+        model, stack = self.model, self.model.stack
         plan = self.cache.resize(self.cache.lengths + 1, tokens=count)
-        tokens = model._embed(ids.to(self.cache.device), plan.positions.long())
+        tokens = model._embed(ids, plan.positions.long())
         a = b = 0
         for i, kind in enumerate(stack.layout):
             if kind == "A":
@@ -141,18 +187,19 @@ class PagedServing:
         else:
             self.sdm.positions.add_(1)
             self.sdm.position += 1
-        self.lengths = [n + 1 for n in self.lengths]
-        return model.output(model.final_norm(tokens))
+        return tokens
 
     @torch.no_grad()
     def release(self, names: Sequence[object]) -> None:
         """Finish requests: their pool rows and K/V pages return, the others keep their order."""
+        self._check_usable()
         gone = [self.requests.index(name) for name in names]
         if len(set(gone)) != len(gone):
             raise ValueError("released requests are named twice")
         if not gone:
             return
         keep = [i for i in range(len(self.requests)) if i not in set(gone)]
+        self._unusable = "a release"
         self.cache.resize([0 if i in set(gone) else n for i, n in enumerate(self.lengths)], tokens=0)
         self.cache = self.cache.with_requests(keep)
         self.sdm.release_and_compact(gone)
@@ -160,6 +207,7 @@ class PagedServing:
         self.lengths = [self.lengths[i] for i in keep]
         if not keep:
             self.sdm = None
+        self._unusable = None
 
     def validate_invariants(self) -> None:
         """Raise on any device error so far, of attention or of the pools, and where pages or rows are lost (synchronises)."""
