@@ -77,14 +77,23 @@ def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
     return t.clone(memory_format=torch.contiguous_format), heads * width, width
 
 
+def _not_capturing(what: str) -> None:
+    """Raise where a buffer that is kept would be made inside a graph capture: its zeroing would be a node of the graph, and
+    calls before the first replay would find it as the allocator left it."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} must be made before the capture: call it once outside")
+
+
 _PROMPT_STATUS: dict[int, torch.Tensor] = {}
 
 
 def prompt_attention_status(device: torch.device) -> torch.Tensor:
     """The device's status word of ``prompt_attention`` calls without one of their own: 0, or ``_lib.ST_WAIT_TIMEOUT`` once a
-    wait inside the kernel gave up and made rows NaN.  Who reads it may zero it."""
+    wait inside the kernel gave up and made rows NaN.  Who reads it may zero it.  It is made at the device's first call,
+    which must not be inside a graph capture."""
     word = _PROMPT_STATUS.get(device.index)
     if word is None:
+        _not_capturing("the status word of prompt attention (prompt_attention_status)")
         word = _PROMPT_STATUS[device.index] = torch.zeros((), dtype=torch.int32, device=device)
     return word
 
@@ -304,9 +313,11 @@ class PagedKVCache:
                workspace: torch.Tensor | None = None) -> torch.Tensor:
         """One query token per request over its cached tokens, ``[requests, heads, head_width]``.
 
-        ``softmax(scale * q . K) V`` in float32 over the ``lengths[b]`` cached tokens, ``scale`` 1 /
-        sqrt(head_width) by default; zeros for a request without tokens.  Calls that may overlap
-        on the GPU need a ``workspace`` each (``new_workspace``).
+        ``softmax(scale * q . K) V`` with float32 sums over the ``lengths[b]`` cached tokens, ``scale`` 1 /
+        sqrt(head_width) by default; zeros for a request without tokens.  16-bit queries have their weights held in
+        float16, float32 ones in two of its parts.  Calls that may overlap on the GPU need a ``workspace`` each
+        (``new_workspace``); the default one is made at the first call for a number of heads, which must not be
+        inside a graph capture.
         """
         shape = queries.shape
         if len(shape) != 3 or shape[0] != self.requests or shape[2] != self.head_width or shape[1] < 1 or shape[1] % self.kv_heads:
@@ -329,7 +340,8 @@ class PagedKVCache:
         return out
 
     def new_workspace(self, heads: int) -> torch.Tensor:
-        """A workspace of ``attend`` for ``heads`` query heads."""
+        """A workspace of ``attend`` for ``heads`` query heads, made outside of any graph capture."""
+        _not_capturing("a workspace of attend (new_workspace)")
         need = _lib.load().cow_kv8_attend_workspace_bytes(self._at, heads)
         if need < 0:
             raise ValueError("heads must be a multiple of kv_heads")

@@ -62,3 +62,25 @@ def test_serving_reports_attention_errors(dev, monkeypatch):  # noqa: F811
     serving.cache.status_word.fill_(_lib.ST_WAIT_TIMEOUT)
     with pytest.raises(RuntimeError, match="gave up"):
         serving.validate_invariants()
+
+
+def test_buffers_that_are_kept_are_not_made_in_a_capture(dev, monkeypatch):  # noqa: F811
+    """Their zeroing would wait for the first replay."""
+    from copy_on_write_sdm_b200 import kv_cache, prompt_attention
+
+    cache = _cache(dev, requests=1, pages=2, kv_heads=1, head_width=32, max_blocks=2)
+    x = torch.randn(2, 5, 1, 32, device=dev)
+    cache.store(x[0], x[1], cache.resize([5], tokens=5))
+    q = torch.randn(1, 2, 32, device=dev)
+    starts = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    monkeypatch.setattr(kv_cache, "_PROMPT_STATUS", {})
+    for early in (lambda: cache.attend(q), lambda: cache.new_workspace(2), lambda: prompt_attention(x[0], x[0], x[1], starts)):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                early()
+    want = cache.attend(q), prompt_attention(x[0], x[0], x[1], starts)  # made here, ready at once
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = cache.attend(q), prompt_attention(x[0], x[0], x[1], starts)
+    graph.replay()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
