@@ -333,6 +333,8 @@ class PagedKVCache:
             workspace = self._workspaces.get(heads)
             if workspace is None:
                 workspace = self._workspaces[heads] = self.new_workspace(heads)
+        elif workspace.dtype != torch.uint8 or workspace.device != self.device or not workspace.is_contiguous():
+            raise ValueError("a workspace is a contiguous uint8 tensor on the cache's device (new_workspace)")
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _call(self.device, "cow_kv8_attend", self._at, layer, q.data_ptr(), q0, q1, code, heads,
               self.head_width ** -0.5 if scale is None else float(scale), out.data_ptr(), workspace.data_ptr(),

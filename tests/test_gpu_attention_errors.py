@@ -84,3 +84,13 @@ def test_buffers_that_are_kept_are_not_made_in_a_capture(dev, monkeypatch):  # n
         got = cache.attend(q), prompt_attention(x[0], x[0], x[1], starts)
     graph.replay()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_workspaces_that_attend_cannot_use(dev):  # noqa: F811
+    cache = _cache(dev, requests=1, pages=1, kv_heads=1, head_width=32, max_blocks=1)
+    q = torch.zeros(1, 2, 32, device=dev)
+    good = cache.new_workspace(2)
+    for bad in (good.cpu(), good.view(torch.float32), torch.zeros(2 * good.numel(), dtype=torch.uint8, device=dev)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            cache.attend(q, workspace=bad)
+    assert cache.attend(q, workspace=good).eq(0).all()
