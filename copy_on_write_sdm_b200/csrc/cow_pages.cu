@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kResizeThreads) cow_pages_resize_kernel(const 
       *reinterpret_cast<int4*>(P.head) = make_int4(0, 0, 0, 0);
     }
     for (int b = self; b <= R; b += threads) P.starts[b] = 0;
-    for (int t = self; t < P.tokens; t += threads) P.slots[t] = P.positions[t] = -1;
+    for (int64_t t = self; t < P.tokens; t += threads) P.slots[t] = P.positions[t] = -1;
     return;  // the same decision in every block: nobody takes a ticket
   }
 
@@ -170,10 +170,12 @@ __global__ void __launch_bounds__(kResizeThreads) cow_pages_resize_kernel(const 
     const int from = max(cur, block * COW_PAGE_TOKENS), to = min(target, (block + 1) * COW_PAGE_TOKENS);
     P.pieces[i] = make_int4(s_new[b] + from - cur, to - from, page_of(b, block), from % COW_PAGE_TOKENS);
   }
-  // kTokensPerThread neighbouring tokens share the search and mostly the page
-  for (int t0 = self * kTokensPerThread; t0 < P.tokens; t0 += threads * kTokensPerThread) {
+  // kTokensPerThread neighbouring tokens share the search and mostly the page.  (In 64 bits: the announced tokens may be near
+  // 2^31, where an int would wrap at the last step.)
+  for (int64_t first = int64_t{self} * kTokensPerThread; first < P.tokens; first += int64_t{threads} * kTokensPerThread) {
+    const int t0 = static_cast<int>(first), end = static_cast<int>(min(first + kTokensPerThread, static_cast<int64_t>(P.tokens)));
     int b = t0 < all.x ? owner_of(s_new, R, t0) : R, block = -1, page = 0;
-    for (int t = t0; t < min(t0 + kTokensPerThread, P.tokens); ++t) {
+    for (int t = t0; t < end; ++t) {
       if (t >= all.x) {
         P.slots[t] = P.positions[t] = -1;
         continue;

@@ -94,3 +94,20 @@ def test_workspaces_that_attend_cannot_use(dev):  # noqa: F811
         with pytest.raises(ValueError, match="workspace"):
             cache.attend(q, workspace=bad)
     assert cache.attend(q, workspace=good).eq(0).all()
+
+
+def test_a_bound_on_new_tokens_near_2_to_the_31(dev):  # noqa: F811
+    """The maps' last steps, of a resize that fits and of one that does not."""
+    tokens = 2**31 - 1
+    cache = _cache(dev, requests=2, pages=3, kv_heads=1, head_width=32, max_blocks=2)
+    for target in ([65, 3], [0, 129]):
+        plan = cache.resize(target, tokens=tokens)
+        new = 68 if target[0] else 0
+        assert plan.starts.tolist() == ([0, 65, 68] if new else [0, 0, 0])
+        for words in (plan.slots, plan.positions):
+            assert bool((words[:new] >= 0).all()) and bool((words[-(1 << 20):] == -1).all()) and int(words[new:].max()) == -1
+        del plan, words
+        torch.cuda.empty_cache()
+    assert int(cache.status_word) and cache.lengths.tolist() == [65, 3]
+    with pytest.raises(ValueError):
+        cache.resize([65, 3], tokens=tokens + 1)
