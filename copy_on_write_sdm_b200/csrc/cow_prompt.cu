@@ -222,15 +222,28 @@ __device__ __forceinline__ void load_matrices_turned(unsigned* r, const uint16_t
                : "memory");
 }
 
-// Adds to a row's output the values of tokens 0..last that are not finite, at two of every eight widths from `from` on.
-__device__ __noinline__ void add_nonfinite_f32(const float* v, int64_t v_token, int last, float* out, int from, int width) {
-  for (int d = from; d < width; d += d % 2 ? 7 : 1) {
-    float sum = out[d];
-    for (int j = 0; j <= last; ++j) {
-      const float x = v[j * v_token + d];
-      if (!(fabsf(x) < INFINITY)) sum += x;
+constexpr int kBadWords = 8;  // 256 spans of key tiles
+
+// Adds to a row's output the values of tokens up to `last` that are not finite, at two of every eight widths from `from` on.
+// They lie in the spans of `per` key tiles that `bad` names, so that few of them cost little however long the prompt is.
+__device__ __noinline__ void add_nonfinite_f32(const float* v, int64_t v_token, const unsigned* bad, int per, int last, float* out, int from,
+                                               int width) {
+  constexpr int kAtOnce = 16;
+  for (int word = 0; word < kBadWords; ++word) {
+    for (unsigned spans = bad[word]; spans != 0; spans &= spans - 1) {
+      const int tile = (32 * word + __ffs(spans) - 1) * per, end = min((tile + per) * kKeys, last + 1);
+      for (int d = from; d < width; d += d % 2 ? 7 : 1) {
+        float sum = 0.f;
+        for (int j = tile * kKeys; j < end; j += kAtOnce) {
+          float x[kAtOnce];
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u) x[u] = j + u < end ? __ldg(v + (j + u) * v_token + d) : 0.f;
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u) sum += fabsf(x[u]) < INFINITY ? 0.f : x[u];
+        }
+        if (sum != 0.f) out[d] += sum;
+      }
     }
-    out[d] = sum;
   }
 }
 
@@ -242,7 +255,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
   uint16_t* s_k = s_q + 3 * S::kRows * S::kStride;         // [3][kKeys][kStride]
   uint16_t* s_v = s_k + 3 * kKeys * S::kStride;             // [3][kKeys][kStride]
   __shared__ Tile s_tile;
-  __shared__ int s_bad;
+  __shared__ unsigned s_bad[kBadWords];  // spans of key tiles with values that are not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int group = P.group, tile_tokens = S::kRows / group, kv_head = blockIdx.x % P.kv_heads, W = P.width;
   const float* Q = static_cast<const float*>(P.q);
@@ -252,16 +265,15 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     TileFinder finder;
     finder.begin(P, tile_tokens);
     const Tile t = finder.find(P, tile_tokens, blockIdx.x / P.kv_heads);
-    if (lane == 0) {
-      s_tile = t;
-      s_bad = 0;
-    }
+    if (lane == 0) s_tile = t;
+    if (lane < kBadWords) s_bad[lane] = 0;
   }
   __syncthreads();
   const Tile t = s_tile;
   if (t.count == 0) return;
   const int here = min(tile_tokens, t.count - t.first);  // tokens of this tile
   const int last = t.first + here;                       // keys 0 .. last - 1
+  const int span = (last - 1) / (kKeys * 32 * kBadWords) + 1;  // key tiles to a bit of s_bad
 
   float4 k[S::kVecs], v[S::kVecs];
   auto load = [&](int j0) {
@@ -322,7 +334,8 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       auto finite = [](float x) { return fabsf(x) < INFINITY ? x : 0.f; };
 #pragma unroll
       for (int i = 0; i < S::kVecs; ++i) v[i] = make_float4(finite(v[i].x), finite(v[i].y), finite(v[i].z), finite(v[i].w));
-      s_bad = 1;
+      const int at = j0 / kKeys / span;
+      atomicOr(&s_bad[at / 32], 1u << (at % 32));
     }
     __syncthreads();  // the last tile is used up
 #pragma unroll
@@ -475,6 +488,9 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
     l0 += __shfl_xor_sync(kFull, l0, x);
     l1 += __shfl_xor_sync(kFull, l1, x);
   }
+  unsigned bad = 0;
+#pragma unroll
+  for (int i = 0; i < kBadWords; ++i) bad |= s_bad[i];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = row0 + 8 * half, token = r / group, query = half ? query1 : query0;
@@ -488,7 +504,7 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
       if (d >= W) continue;
       *reinterpret_cast<float2*>(out + d) = make_float2(o[i][2 * half] * inv, o[i][2 * half + 1] * inv);
     }
-    if (s_bad) add_nonfinite_f32(V + t.begin * P.v_token, P.v_token, query, out, 2 * c, W);
+    if (bad) add_nonfinite_f32(V + t.begin * P.v_token, P.v_token, s_bad, span, query, out, 2 * c, W);
   }
 }
 

@@ -110,3 +110,22 @@ def test_the_largest_values_of_the_type(dev):  # noqa: F811
     v[:] = 0.99 * torch.finfo(torch.float32).min
     got = prompt_attention(q, k, v, device_starts)
     torch.testing.assert_close(got, torch.full_like(got, 0.99 * torch.finfo(torch.float32).min), rtol=2.0**-19, atol=0.0)
+
+
+def test_values_that_are_not_finite_in_a_long_prompt(dev):  # noqa: F811
+    """Few of them, in spans of more than one key tile; each row has the sum of those that it sees."""
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    q, k, v, _, device_starts = _inputs(dev, [17000, 100], 1, 1, 32, torch.float32, 11)
+    clean = prompt_attention(q, k, v, device_starts)
+    inf, nan = float("inf"), float("nan")
+    bad = {(700, 3): inf, (9001, 3): inf, (12000, 3): -inf, (16990, 4): -inf, (5, 5): nan, (17050, 6): inf}
+    for (token, d), x in bad.items():
+        v[token, 0, d] = x
+    got = prompt_attention(q, k, v, device_starts)
+    want = clean.clone()
+    for (token, d), x in bad.items():
+        want[token:17000 if token < 17000 else None, 0, d] += x
+    same = want.isfinite()
+    torch.testing.assert_close(got[~same], want[~same], rtol=0, atol=0, equal_nan=True)
+    torch.testing.assert_close(got[same], clean[same], rtol=0, atol=0)
