@@ -12,6 +12,8 @@
 
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "cow_common.cuh"
 
 namespace {
@@ -1129,7 +1131,8 @@ int cow_kv8_store(const cow_kv_pages* cache, int32_t layer, const void* keys, in
   if (!cache || !valid_dtype(dtype) || !plan || !aligned16(plan) || layer < 0 || layer >= cache->layers || tokens < 0)
     return COW_ERR_INVALID;
   if (!shape_ok(cache)) return COW_ERR_UNSUPPORTED;
-  if (tokens == 0) return COW_OK;
+  const int64_t pieces = std::min(tokens, tokens / kPage + 2 * cache->requests);  // at most; none without requests
+  if (pieces == 0) return COW_OK;
   if (!rows_ok(keys, key_token_stride, key_head_stride, dtype) ||
       !rows_ok(values, value_token_stride, value_head_stride, dtype) || !cache->key_codes || !cache->value_codes ||
       !cache->key_scales || !cache->value_scales)
@@ -1142,7 +1145,6 @@ int cow_kv8_store(const cow_kv_pages* cache, int32_t layer, const void* keys, in
                 {key_token_stride * size, value_token_stride * size},
                 {key_head_stride * size, value_head_stride * size},
                 plan, cache->kv_heads, static_cast<int32_t>(cache->pages)};
-  const int64_t pieces = (tokens < tokens / kPage + 2 * cache->requests) ? tokens : tokens / kPage + 2 * cache->requests;
   const dim3 grid(static_cast<unsigned>(pieces), static_cast<unsigned>(cache->kv_heads), 2);
   if (dtype == COW_F32) launch_store<COW_F32>(P, cache->width, grid, as_stream(stream));
   else if (dtype == COW_BF16) launch_store<COW_BF16>(P, cache->width, grid, as_stream(stream));

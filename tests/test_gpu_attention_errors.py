@@ -111,3 +111,13 @@ def test_a_bound_on_new_tokens_near_2_to_the_31(dev):  # noqa: F811
     assert int(cache.status_word) and cache.lengths.tolist() == [65, 3]
     with pytest.raises(ValueError):
         cache.resize([65, 3], tokens=tokens + 1)
+
+
+def test_store_for_no_request(dev):  # noqa: F811
+    """Room for tokens in the plan of a cache without requests: nothing is stored, nothing raised."""
+    cache = _cache(dev, requests=0, pages=1, kv_heads=1, head_width=32, max_blocks=1)
+    for tokens in (0, 5, 200):
+        x = torch.ones(tokens, 1, 32, device=dev)
+        cache.store(x, x, cache.resize([], tokens=tokens))
+    assert not cache.key_pages.view(torch.uint8).any()
+    cache.validate_invariants()
