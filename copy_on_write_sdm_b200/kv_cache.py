@@ -23,6 +23,7 @@ from dataclasses import dataclass, field, replace
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -63,7 +64,7 @@ def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
     copy where it is not so), and its strides; those of a dimension of one are made up."""
     if not t.is_cuda:
         _lib.require_cuda(t, what)
-    if t.requires_grad and torch.is_grad_enabled():
+    if (t.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
         raise ValueError(f"{what} asks for a gradient: the serving attention has no backward pass")
     n, heads, width = t.shape
     s0, s1, s2 = t.stride()

@@ -121,3 +121,21 @@ def test_store_for_no_request(dev):  # noqa: F811
         cache.store(x, x, cache.resize([], tokens=tokens))
     assert not cache.key_pages.view(torch.uint8).any()
     cache.validate_invariants()
+
+
+def test_forward_mode_tangents_are_refused(dev):  # noqa: F811
+    """As inputs that ask for a gradient are: they would be dropped."""
+    from torch.autograd import forward_ad
+
+    from copy_on_write_sdm_b200 import prompt_attention
+
+    cache = _cache(dev, requests=1, pages=1, kv_heads=1, head_width=32, max_blocks=1)
+    x = torch.randn(3, 1, 32, device=dev)
+    starts = torch.tensor([0, 3], dtype=torch.int32, device=dev)
+    plan = cache.resize([3], tokens=3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: prompt_attention(x, dual, x, starts), lambda: cache.store(x, dual, plan), lambda: cache.attend(dual[:1])):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        prompt_attention(x, x, x, starts)  # inputs without one pass
