@@ -19,6 +19,7 @@ neither synchronises nor allocates anything but its results and, once, its works
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass, field, replace
 from typing import Sequence
 
@@ -357,8 +358,14 @@ class PagedKVCache:
     def with_requests(self, keep: torch.Tensor | Sequence[int], *, new: int = 0) -> "PagedKVCache":
         """The cache with the request slots ``keep``, in their order, and ``new`` empty ones after
         them: same pages and stack.  Requests left out must have been resized to 0 (their pages
-        would be lost).  The old object is not used again."""
-        keep = torch.as_tensor(keep, dtype=torch.int64, device=self.device)
+        would be lost).  The old object is not used again.  (``keep`` is checked on the host: one on the device is copied there.)"""
+        try:
+            keep = [operator.index(i) for i in (keep.tolist() if isinstance(keep, torch.Tensor) else keep)]
+        except TypeError:
+            raise ValueError("kept requests must be a vector of whole numbers") from None
+        if len(set(keep)) != len(keep) or not all(0 <= i < self.requests for i in keep):
+            raise ValueError(f"kept requests must be different ones of 0 .. {self.requests - 1}")
+        keep = torch.tensor(keep, dtype=torch.int64, device=self.device)
         total = keep.shape[0] + new
         if new < 0 or total > MAX_REQUESTS or total * self.max_blocks >= 1 << 25:
             raise ValueError("the K/V cache exceeds the compiled limits (8192 requests, 2^25 table entries)")

@@ -90,7 +90,7 @@ class PagedServing:
             self._unusable = "an admission and its undoing"
             if self.cache is not cache:  # pages and rows taken so far go back
                 self.cache.resize(self.lengths + [0] * len(counts), tokens=0)
-                self.cache = self.cache.with_requests(torch.arange(live, device=cache.device))
+                self.cache = self.cache.with_requests(range(live))
             self.sdm = sdm
             if sdm is not None:
                 if sdm.batch > live:
@@ -106,7 +106,7 @@ class PagedServing:
 
     def _admit(self, ids: torch.Tensor, counts: list[int], live: int) -> torch.Tensor:
         model, stack = self.model, self.model.stack
-        self.cache = self.cache.with_requests(torch.arange(live, device=self.cache.device), new=len(counts))
+        self.cache = self.cache.with_requests(range(live), new=len(counts))
         plan = self.cache.resize(self.lengths + counts, tokens=sum(counts))
         tokens = model._embed(ids, plan.positions.long())
 

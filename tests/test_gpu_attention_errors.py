@@ -139,3 +139,17 @@ def test_forward_mode_tangents_are_refused(dev):  # noqa: F811
             with pytest.raises(ValueError, match="gradient"):
                 call()
         prompt_attention(x, x, x, starts)  # inputs without one pass
+
+
+def test_requests_that_cannot_be_kept(dev):  # noqa: F811
+    """A slot that is not there would be an index out of range on the device, one kept twice two owners of its pages."""
+    cache = _cache(dev, requests=3, pages=3, kv_heads=1, head_width=32, max_blocks=1)
+    cache.resize([1, 2, 3], tokens=6)
+    for keep in ([3], [-1], [0, 0], [0.5], torch.tensor([0, 7]), torch.tensor([1, 1], device=dev), torch.tensor([[0]])):
+        with pytest.raises(ValueError):
+            cache.with_requests(keep)
+    plan = cache.resize([1, 2, 0], tokens=0)
+    assert plan.starts.tolist() == [0, 0, 0, 0]
+    kept = cache.with_requests(torch.tensor([1, 0], device=dev), new=1)
+    assert kept.lengths.tolist() == [2, 1, 0]
+    kept.validate_invariants()
