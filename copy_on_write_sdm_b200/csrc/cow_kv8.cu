@@ -397,9 +397,10 @@ constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = 32 * kAttendWarps;
 constexpr int kAttendHeads = 8;   // query heads of one block: the matrix instruction's columns
 constexpr int kJoin = 8;            // parts a warp of the second kernel reads at once
-// Threads of a block of the second kernel: few pairs have many parts each, and many pairs are best all at once
-// (32 pairs of 180 parts: 19 us with 128 threads; 512 pairs of 4: 16 us with 256).
-constexpr int kJoinFewPairs = 148, kJoinThreadsFew = 512, kJoinThreadsMany = 128;
+// Threads of a block of the second kernel: few pairs have many parts each, and many pairs are best all at once.  Both kernels,
+// 512,000 tokens of 8 heads of 128, with 512 / 128 threads: 32 pairs 180 / 196 us, 64 186 / 192, 128 187 / 183, 144 185 / 179,
+// 256 189 / 175, 512 206 / 182.
+constexpr int kJoinFewPairs = 96, kJoinThreadsFew = 512, kJoinThreadsMany = 128;
 constexpr int kJoinColumns = 148 * 4;
 constexpr int kAlignedPages = 16;  // four pages a warp: less than a join through global memory takes
 constexpr float kProbShift = 8.f;  // probabilities are held times 2^8: more of f16's range below the largest
