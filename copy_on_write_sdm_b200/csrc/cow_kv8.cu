@@ -386,11 +386,12 @@ __global__ void __launch_bounds__(kReadThreads) cow_kv8_read_kernel(const __grid
 //   contraction is 1/10 of what this instruction sustains at the memory's rate.
 //   Queries are scaled per head by a power of two into f16's range; f32 ones are
 //   held as two f16 parts (22 bits), and so are their probabilities.
+//   (Widths of a query 2^28 below its largest keep fewer bits: f16's last place lies 2^38 below.)
 // * running maximum, sum and output of the softmax stay in f32 registers.  A page's weights are taken relative to its
 //   own largest score, so that f16 holds them whatever the others' are; the page's sums join the running ones in f32, where
 //   the difference of the maxima and the value scale are one factor.
-// Measured (32/8 heads of 128, bf16): 64 requests of 64 to 4,096 tokens 64 us (4.4 TB/s: 54 us of it the first kernel),
-// 4 of 65,536 102 us (5.3 TB/s, the first kernel 5.9); 16 of 256 to 512 tokens, 4 heads of 32, f32: 9.8 us, where
+// Measured (32/8 heads of 128, bf16): 64 requests of 64 to 4,096 tokens 65 us (4.3 TB/s: 54 us of it the first kernel),
+// 4 of 65,536 102-104 us (5.2 TB/s, the first kernel 5.9); 16 of 256 to 512 tokens, 4 heads of 32, f32: 9 us, where
 // latency is all: 1.7 us until the lengths are scanned, 3.5 us for two pages, 1 us for the warps to meet.
 
 constexpr int kAttendWarps = 4;

@@ -533,9 +533,9 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 // them have them added at the end.
 //
 // A block stays and takes tile after tile: loads and scores of the next begin under the end of the last.
-// Measured (bf16): 2 x 8,192 tokens, 32/8 heads of 128: 0.95-1.03 ms, 1,070-1,160 TFLOP/s back to back under the power
-// cap (a cuBLAS product sustains 1,384 there, 1,658 in a burst); 32 requests of 64 to 2,048, 16/4 heads of 64: 193 us,
-// 533 TFLOP/s; 21 of 1 to 777, 14/2 heads of 96 (f16): 35 us.  Bound: the chain from a tile's scores through its softmax
+// Measured (bf16): 2 x 8,192 tokens, 32/8 heads of 128: 1.00-1.03 ms, 1,070-1,100 TFLOP/s back to back under the power
+// cap (a cuBLAS product sustains 1,384 there, 1,658 in a burst); 32 requests of 64 to 2,048, 16/4 heads of 64: 188-193 us,
+// 530-550 TFLOP/s; 21 of 1 to 777, 14/2 heads of 96 (f16): 35-36 us.  Bound: the chain from a tile's scores through its softmax
 // (1,750 cycles) and the two products (768 after the first half of P) back to its next scores, 2,900 cycles for the
 // 2,048 of tensor work of both tiles; for narrow heads the 48 special-function and 370 other instructions of a warp for
 // 32 rows of 64 keys; for short prompts what a tile costs beside its key tiles, 4,000 cycles (last products,
@@ -544,8 +544,9 @@ __global__ void __launch_bounds__(F32Shape<D>::kThreads, D > 64 ? 1 : D > 32 ? 2
 // (they fall into step with each other: 4,200), three score tiles in turn for widths to 64 (the softmax is the
 // bound: no change), the output given up as soon as it is in registers (the same: 1 % slower), masked tiles looked
 // through only where some row does not see them, and from a step earlier (no change).
-// Of eight pairs of weights, two come from the polynomial (0: 395,000 cycles for 8,192 tokens of
-// 16/4 heads of 64, 2: 354,000, 3: 369,000).
+// Of eight pairs of weights, two come from the polynomial.  4,096 tokens of 16/4 heads of 32 / 64 / 96 / 128, us, with none,
+// one, two and three: bf16 57 60 65 71, 53 56 60 64, 54 56 59 63, 56 58 62 67; f16 53 60 64 70, 52 56 61 65, 54 58 62 65,
+// 56 61 65 67.
 // Every wait is bounded; one that gives up sets a status bit and ends the block, all its rows NaN.
 
 constexpr int kTcThreads = 640;
